@@ -53,7 +53,17 @@ enum swcb200_precision {
 };
 
 enum swcb200_dtype { SWCB200_F32 = 0, SWCB200_BF16 = 1, SWCB200_I32 = 2 };
-enum swcb200_act { SWCB200_ACT_NONE = 0, SWCB200_ACT_RELU = 1, SWCB200_ACT_TANH = 2 };
+enum swcb200_act {
+    SWCB200_ACT_NONE = 0,
+    SWCB200_ACT_RELU = 1,
+    SWCB200_ACT_TANH = 2,
+    /* swcb200_fc_bf16_residual only: */
+    SWCB200_ACT_GELU = 3,      /* v * Phi(v), Phi the normal distribution function          */
+    SWCB200_ACT_GELU_TANH = 4, /* v/2 * (1 + tanh(sqrt(2/pi) * (v + 0.044715 v^3)))          */
+    SWCB200_ACT_SILU = 5       /* v / (1 + exp(-v))                                          */
+};
+/* norms of swcb200_norm_residual */
+enum swcb200_norm_kind { SWCB200_NORM_NONE = 0, SWCB200_NORM_RMS = 1, SWCB200_NORM_LAYER = 2 };
 
 /* ------------------------------------------------------------------ context */
 
@@ -229,6 +239,66 @@ int swcb200_conv2d_bf16(swcb200_ctx *ctx, void *output, const void *input, const
 int swcb200_maxpool_bf16(swcb200_ctx *ctx, const void *input, void *output, const size_t *idims,
                          const size_t *odims, const size_t *kernels, const size_t *strides,
                          const size_t *pads);
+
+/* ------------------------------------------------- transformer blocks
+ * The forward pass of a block around the same bf16 rows; the reference has no such nodes. */
+
+/* C[m,n] = residual[m,n] + scale * act(A[m,k] . Wp[n,k]^T + bias[n]).  A, Wp (swcb200_pack_weight_bf16)
+ * bf16 under the rules of swcb200_fc_bf16: 16-byte aligned, lda and ldw multiples of 8; C and the
+ * residual fp32 or bf16 at any alignment and pitch.  Sums, bias, activation and residual are fp32,
+ * rounded once at the store.  The residual may be C itself (same pointer, type and leading
+ * dimension), any other overlap of the two is refused.  Any m from one row on: few rows divide k
+ * over a cluster of CTAs. */
+typedef struct swcb200_fc_epilogue {
+    const float *bias; /* [n] or NULL */
+    int act;           /* enum swcb200_act, all of them */
+    float scale;
+    const void *residual; /* [m,n] or NULL */
+    int residual_dtype, ld_residual;
+} swcb200_fc_epilogue;
+int swcb200_fc_bf16_residual(swcb200_ctx *ctx, int m, int n, int k, const void *a_bf16, int lda,
+                             const void *wp_bf16, int ldw, const swcb200_fc_epilogue *ep, void *c,
+                             int c_dtype, int ldc);
+
+/* One norm over the columns of a row.  RMS: v * weight / sqrt(mean(v^2) + eps) + bias; LAYER:
+ * (v - mean) / sqrt(var + eps) * weight + bias with the biased variance.  weight and bias fp32
+ * [cols], NULL for 1 and 0. */
+typedef struct swcb200_norm {
+    int kind; /* enum swcb200_norm_kind; NONE: absent */
+    const float *weight, *bias;
+    float eps; /* >= 0 */
+} swcb200_norm;
+/* What lies between two blocks, for every row:
+ *     t = residual + scale * gate * post(x)      -> sum
+ *     y = pre(t)                                 -> y
+ * Tensors [rows, cols], SWCB200_F32 or SWCB200_BF16 each, leading dimensions in elements.  NULL
+ * leaves residual, gate or sum out (sum or y has to be there); y and pre go together.  Row r is
+ * multiplied by gate row r / gate_rows, or every row by the one gate row where gate_rows is 0.
+ * All arithmetic is fp32; t goes into pre() unrounded.  sum and y may each be x or residual in
+ * place (same pointer, type and leading dimension), other overlaps are refused.  Rows of one call
+ * at any alignment; 128- and 256-bit accesses where all pointers allow them.  cols <= 16384. */
+typedef struct swcb200_norm_block {
+    const void *x;
+    int x_dtype;
+    size_t ldx;
+    swcb200_norm post;
+    const void *gate;
+    int gate_dtype;
+    size_t ld_gate;
+    long long gate_rows;
+    float scale;
+    const void *residual;
+    int residual_dtype;
+    size_t ld_residual;
+    void *sum;
+    int sum_dtype;
+    size_t ld_sum;
+    swcb200_norm pre;
+    void *y;
+    int y_dtype;
+    size_t ldy;
+} swcb200_norm_block;
+int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, const swcb200_norm_block *block);
 
 /* ---------------------------------------------------- partitioned graphs
  * NCCL over NVLink in place of the MPI text ParallelCodegen prints

@@ -4,9 +4,11 @@ The product is the C-ABI library ``libswc_b200.so`` (``include/swc_b200.h``); th
 loads it and mirrors the reference's kernel interface on torch CUDA tensors (``kernels.Backend``).
 """
 from . import _lib
-from ._lib import (ACT_NONE, ACT_RELU, ACT_TANH, BF16, F32, STRICT_F32, TC_BF16, SwcError)
+from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_RELU, ACT_SILU, ACT_TANH, BF16, F32, NORM_LAYER, NORM_RMS, STRICT_F32,
+                   TC_BF16, SwcError)
 
-__all__ = ["Backend", "_lib", "SwcError", "STRICT_F32", "TC_BF16", "F32", "BF16", "ACT_NONE", "ACT_RELU", "ACT_TANH"]
+__all__ = ["Backend", "_lib", "SwcError", "STRICT_F32", "TC_BF16", "F32", "BF16", "ACT_NONE", "ACT_RELU", "ACT_TANH",
+           "ACT_GELU", "ACT_GELU_TANH", "ACT_SILU", "NORM_RMS", "NORM_LAYER"]
 
 
 def __getattr__(name):

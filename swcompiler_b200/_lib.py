@@ -13,7 +13,8 @@ OK, ERR_BAD_ARG, ERR_BAD_SHAPE, ERR_MISALIGNED, ERR_UNSUPPORTED, ERR_CUDA, ERR_N
     ERR_TOO_LARGE = range(10)
 STRICT_F32, TC_BF16 = 0, 1
 F32, BF16, I32 = 0, 1, 2
-ACT_NONE, ACT_RELU, ACT_TANH = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_TANH, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(6)
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
 MAX_PEERS = 8
 
 _lib = None

@@ -38,6 +38,9 @@ int swc_scratch(swcb200_ctx *ctx, size_t bytes, void **out);
 int swc_cast_pad_rows(swcb200_ctx *ctx, const float *a, int m, int k, int lda, void *out_bf16, int ldo);
 // fp32 W[k, n] with pitch ldb -> bf16 Wp[n, k] with pitch ldo
 int swc_pack_weight_padded(swcb200_ctx *ctx, const float *w, int k, int n, int ldb, void *wp_bf16, int ldo);
+// whether two tensors of `rows` rows (pitch and width in bytes, width <= pitch) share a byte; exact for equal pitches, else
+// true whenever their address ranges meet
+bool swc_rows_overlap(const void *a, size_t a_pitch, size_t a_width, const void *b, size_t b_pitch, size_t b_width, size_t rows);
 
 #define SWC_REQUIRE(ctx, cond, status, ...)                         \
     do {                                                            \

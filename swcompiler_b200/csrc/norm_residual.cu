@@ -1,0 +1,365 @@
+// The rows between two blocks of a transformer, in one pass:
+//     t = residual + scale * gate * post(x)        sum <- t
+//     y = pre(t)
+// post and pre are RMS norms (x * w / sqrt(mean(x^2) + eps)), layer norms ((x - mean) / sqrt(var + eps) * w + b, biased
+// variance) or absent.
+//
+// What bounds it: the bytes of x, residual, sum and y; about ten operations per element.  So a row is read once, held in
+// registers as fp32 through up to four row sums, and written once.  The layer norm's variance is the mean of
+// (t - mean)^2 over the registers (no E[t^2] - mean^2, which cancels).  pre() reads t before it is rounded to sum's type:
+// the value is there, and rounding it first would only add an error to y.
+//
+// Layout: a row belongs to `tpr` threads.  Up to 32 of them (rows of at most 1024 elements) are a part of one warp and the
+// sums are shuffles; above that the row is a CTA of its own.  A thread holds at most 32 elements of a row.  Rows whose
+// tensors are all aligned move in chunks of 8 elements (16 bytes of bf16, one 32-byte access of fp32); other rows one
+// element per access, neighbouring threads at neighbouring elements.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kMaxThreads = 512;  // 128 registers each: 64 hold the row and its residual
+constexpr int kMaxCols = kMaxThreads * 32;
+
+struct NormParams {
+    const float *w, *b;
+    float eps;
+    int kind;
+};
+
+struct RowParams {
+    const void *x, *residual, *gate;
+    void *sum, *y;
+    size_t ldx, ldr, ldg, lds, ldy;  // elements
+    int x16, r16, g16, s16, y16;     // 1: bf16, 0: fp32
+    long long rows, gate_rows;
+    int cols, tpr;
+    float scale, inv_cols;
+    NormParams post, pre;
+};
+
+__device__ __forceinline__ void load8(const void *p, size_t i, bool is16, float (&v)[8]) {
+    if (is16) {
+        uint32_t r[4];
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "l"(reinterpret_cast<const __nv_bfloat16 *>(p) + i));
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[2 * j] = __uint_as_float(r[j] << 16);
+            v[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
+        }
+    } else {
+        asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(reinterpret_cast<const float *>(p) + i));
+    }
+}
+
+__device__ __forceinline__ void store8(void *p, size_t i, bool is16, const float (&v)[8]) {
+    if (is16) {
+        uint32_t r[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            r[j] = *reinterpret_cast<uint32_t *>(&h);
+        }
+        asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(reinterpret_cast<__nv_bfloat16 *>(p) + i),
+                     "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                     : "memory");
+    } else {
+        asm volatile("st.global.L1::no_allocate.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                         reinterpret_cast<float *>(p) + i),
+                     "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+    }
+}
+
+// the per-channel vectors: every row reads them, so they stay in L1
+__device__ __forceinline__ void vector8(const float *p, int i, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p + i)), b = __ldg(reinterpret_cast<const float4 *>(p + i) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+
+// sum over the row's threads; every thread gets it
+template <bool kCta>
+__device__ __forceinline__ float row_sum(float v, int tpr, float *red) {
+    if (!kCta) {
+        for (int o = tpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        return v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? red[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+
+// t <- norm(t) over the kN * kVec elements of this thread; element e of chunk i is column (i * tpr + tid) * kVec + e
+template <int kVec, int kN, bool kCta>
+__device__ __forceinline__ void norm_row(const NormParams &n, const RowParams &p, float (&t)[kN * kVec], int tid, float *red) {
+    if (n.kind == SWCB200_NORM_LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < kN * kVec; j++) s += t[j];  // elements past the row are 0
+        const float mean = row_sum<kCta>(s, p.tpr, red) * p.inv_cols;
+#pragma unroll
+        for (int i = 0; i < kN; i++)
+#pragma unroll
+            for (int e = 0; e < kVec; e++)
+                t[i * kVec + e] = (i * p.tpr + tid) * kVec + e < p.cols ? t[i * kVec + e] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < kN * kVec; j++) q = fmaf(t[j], t[j], q);
+    const float rstd = 1.0f / sqrtf(row_sum<kCta>(q, p.tpr, red + 32) * p.inv_cols + n.eps);
+#pragma unroll
+    for (int i = 0; i < kN; i++) {
+        const int c = (i * p.tpr + tid) * kVec;
+        if (c >= p.cols) continue;
+        if (kVec == 8) {
+            float w[8];
+            if (n.w) vector8(n.w, c, w);
+#pragma unroll
+            for (int e = 0; e < kVec; e++) t[i * kVec + e] *= n.w ? rstd * w[e % 8] : rstd;
+            if (n.b) {
+                vector8(n.b, c, w);
+#pragma unroll
+                for (int e = 0; e < kVec; e++) t[i * kVec + e] += w[e % 8];
+            }
+        } else {
+            t[i] *= n.w ? rstd * __ldg(n.w + c) : rstd;
+            if (n.b) t[i] += __ldg(n.b + c);
+        }
+    }
+}
+
+__device__ __forceinline__ float load1(const void *p, size_t i, bool is16) {
+    return is16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]) : reinterpret_cast<const float *>(p)[i];
+}
+__device__ __forceinline__ void store1(void *p, size_t i, bool is16, float v) {
+    if (is16)
+        reinterpret_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+    else
+        reinterpret_cast<float *>(p)[i] = v;
+}
+
+// kVec elements of chunk c of a row
+template <int kVec>
+__device__ __forceinline__ void load_chunk(const void *p, size_t i, bool is16, float (&v)[kVec]) {
+    if constexpr (kVec == 8)
+        load8(p, i, is16, v);
+    else
+        v[0] = load1(p, i, is16);
+}
+
+template <int kVec, int kN, bool kCta>
+__global__ void __launch_bounds__(kCta ? kMaxThreads : 128) norm_residual_kernel(const RowParams p) {
+    __shared__ float red[128];  // one part for each of the four row sums: no barrier between reading one and writing the next
+    const int tid = kCta ? threadIdx.x : threadIdx.x & (p.tpr - 1);
+    const int rows_per_cta = kCta ? 1 : blockDim.x / p.tpr;
+    const long long row = (long long)blockIdx.x * rows_per_cta + (kCta ? 0 : threadIdx.x / p.tpr);
+    // threads of a row past the last one keep their lanes in the shuffles and touch no memory
+    const int cols = row < p.rows ? p.cols : 0;
+    float t[kN * kVec], r[kN * kVec];
+#pragma unroll
+    for (int i = 0; i < kN; i++) {
+        const int c = (i * p.tpr + tid) * kVec;
+        float v[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; e++) v[e] = 0.f;
+        if (c < cols) load_chunk<kVec>(p.x, (size_t)row * p.ldx + c, p.x16, v);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) t[i * kVec + e] = v[e];
+    }
+    if (p.residual) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int c = (i * p.tpr + tid) * kVec;
+            float v[kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; e++) v[e] = 0.f;
+            if (c < cols) load_chunk<kVec>(p.residual, (size_t)row * p.ldr + c, p.r16, v);
+#pragma unroll
+            for (int e = 0; e < kVec; e++) r[i * kVec + e] = v[e];
+        }
+    }
+    if (p.post.kind) norm_row<kVec, kN, kCta>(p.post, p, t, tid, red);
+#pragma unroll
+    for (int j = 0; j < kN * kVec; j++) t[j] *= p.scale;
+    if (p.gate) {
+        const size_t base = p.gate_rows ? (size_t)(row / p.gate_rows) * p.ldg : 0;
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int c = (i * p.tpr + tid) * kVec;
+            if (c >= cols) continue;
+            float v[kVec];
+            if constexpr (kVec == 8) {
+                if (!p.g16)
+                    vector8(reinterpret_cast<const float *>(p.gate) + base, c, v);
+                else
+                    load8(p.gate, base + c, true, v);
+            } else {
+                v[0] = load1(p.gate, base + c, p.g16);
+            }
+#pragma unroll
+            for (int e = 0; e < kVec; e++) t[i * kVec + e] *= v[e];
+        }
+    }
+    if (p.residual) {
+#pragma unroll
+        for (int j = 0; j < kN * kVec; j++) t[j] += r[j];
+    }
+    if (p.sum) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int c = (i * p.tpr + tid) * kVec;
+            if (c >= cols) continue;
+            if constexpr (kVec == 8) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = t[i * 8 + e];
+                store8(p.sum, (size_t)row * p.lds + c, p.s16, v);
+            } else {
+                store1(p.sum, (size_t)row * p.lds + c, p.s16, t[i]);
+            }
+        }
+    }
+    if (p.pre.kind) {
+        norm_row<kVec, kN, kCta>(p.pre, p, t, tid, red + 64);
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int c = (i * p.tpr + tid) * kVec;
+            if (c >= cols) continue;
+            if constexpr (kVec == 8) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = t[i * 8 + e];
+                store8(p.y, (size_t)row * p.ldy + c, p.y16, v);
+            } else {
+                store1(p.y, (size_t)row * p.ldy + c, p.y16, t[i]);
+            }
+        }
+    }
+}
+
+template <int kVec, bool kCta>
+void launch(int n, unsigned grid, int threads, cudaStream_t s, const RowParams &p) {
+    constexpr int k = kVec == 8 ? 1 : 8;  // chunks of one element come in eights
+    if (n <= k)
+        norm_residual_kernel<kVec, k, kCta><<<grid, threads, 0, s>>>(p);
+    else if (n <= 2 * k)
+        norm_residual_kernel<kVec, 2 * k, kCta><<<grid, threads, 0, s>>>(p);
+    else
+        norm_residual_kernel<kVec, 4 * k, kCta><<<grid, threads, 0, s>>>(p);
+}
+
+bool known_dtype(int d) { return d == SWCB200_F32 || d == SWCB200_BF16; }
+
+}  // namespace
+
+bool swc_rows_overlap(const void *a, size_t a_pitch, size_t a_width, const void *b, size_t b_pitch, size_t b_width, size_t rows) {
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    const uintptr_t a1 = a0 + (rows - 1) * a_pitch + a_width, b1 = b0 + (rows - 1) * b_pitch + b_width;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (rows == 1 || a_pitch != b_pitch) return true;  // ranges meet: taken as an overlap
+    const size_t d = b0 >= a0 ? (b0 - a0) % a_pitch : (a_pitch - (a0 - b0) % a_pitch) % a_pitch;
+    return d < a_width || d + b_width > a_pitch;  // else columns of one tensor side by side
+}
+
+SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, const swcb200_norm_block *d) {
+    SWC_CTX(ctx);
+    SWC_REQUIRE(ctx, d != nullptr, SWCB200_ERR_BAD_ARG, "norm_residual: null description");
+    SWC_REQUIRE(ctx, cols >= 1, SWCB200_ERR_BAD_ARG, "norm_residual: bad column count %d", cols);
+    SWC_REQUIRE(ctx, cols <= kMaxCols && rows <= 0x7fffffffu, SWCB200_ERR_TOO_LARGE,
+                "norm_residual: at most %d columns and 2^31 - 1 rows", kMaxCols);
+    const swcb200_norm *norms[2] = {&d->post, &d->pre};
+    for (const swcb200_norm *n : norms) {
+        SWC_REQUIRE(ctx, n->kind >= SWCB200_NORM_NONE && n->kind <= SWCB200_NORM_LAYER, SWCB200_ERR_BAD_ARG,
+                    "norm_residual: unknown norm %d", n->kind);
+        SWC_REQUIRE(ctx, n->kind == SWCB200_NORM_NONE || n->eps >= 0.f, SWCB200_ERR_BAD_ARG, "norm_residual: negative eps");
+    }
+    SWC_REQUIRE(ctx, known_dtype(d->x_dtype) && (!d->residual || known_dtype(d->residual_dtype)) &&
+                (!d->gate || known_dtype(d->gate_dtype)) && (!d->sum || known_dtype(d->sum_dtype)) &&
+                (!d->y || known_dtype(d->y_dtype)), SWCB200_ERR_BAD_ARG, "norm_residual: tensors are fp32 or bf16");
+    SWC_REQUIRE(ctx, (d->y != nullptr) == (d->pre.kind != SWCB200_NORM_NONE), SWCB200_ERR_BAD_ARG,
+                "norm_residual: y and the norm that writes it go together");
+    SWC_REQUIRE(ctx, d->gate_rows >= 0, SWCB200_ERR_BAD_ARG, "norm_residual: negative gate_rows");
+    if (rows == 0) return SWCB200_OK;
+    SWC_REQUIRE(ctx, d->x && (d->sum || d->y), SWCB200_ERR_BAD_ARG, "norm_residual: null tensor");
+    const size_t c = (size_t)cols;
+    SWC_REQUIRE(ctx, rows == 1 || (d->ldx >= c && (!d->residual || d->ld_residual >= c) && (!d->sum || d->ld_sum >= c) &&
+                                   (!d->y || d->ldy >= c) && (!d->gate || !d->gate_rows || d->ld_gate >= c)),
+                SWCB200_ERR_BAD_SHAPE, "norm_residual: leading dimension too small");
+    // an output may be one of the inputs in place (a thread reads what it overwrites before it writes); nothing else may overlap
+    struct Tensor {
+        const void *p;
+        size_t ld, size, rows;
+    };
+    const auto size = [](int dt) { return dt == SWCB200_BF16 ? (size_t)2 : (size_t)4; };
+    const Tensor in[3] = {{d->x, d->ldx, size(d->x_dtype), rows},
+                          {d->residual, d->ld_residual, size(d->residual_dtype), rows},
+                          {d->gate, d->ld_gate, size(d->gate_dtype), d->gate_rows ? (rows - 1) / (size_t)d->gate_rows + 1 : 1}};
+    const Tensor out[2] = {{d->sum, d->ld_sum, size(d->sum_dtype), rows}, {d->y, d->ldy, size(d->y_dtype), rows}};
+    const auto meet = [&](const Tensor &a, const Tensor &b) {
+        if (!a.p || !b.p) return false;
+        if (a.rows == b.rows)
+            return swc_rows_overlap(a.p, a.ld * a.size, c * a.size, b.p, b.ld * b.size, c * b.size, a.rows);
+        const char *a0 = (const char *)a.p, *b0 = (const char *)b.p;
+        return a0 < b0 + ((b.rows - 1) * b.ld + c) * b.size && b0 < a0 + ((a.rows - 1) * a.ld + c) * a.size;
+    };
+    for (const Tensor &o : out)
+        for (int i = 0; i < 3; i++) {
+            const bool in_place = i < 2 && o.p == in[i].p && o.size == in[i].size && (rows == 1 || o.ld == in[i].ld);
+            SWC_REQUIRE(ctx, in_place || !meet(o, in[i]), SWCB200_ERR_BAD_ARG,
+                        "norm_residual: an output overlaps an input without being the same tensor");
+        }
+    SWC_REQUIRE(ctx, !meet(out[0], out[1]), SWCB200_ERR_BAD_ARG, "norm_residual: the two outputs overlap");
+
+    RowParams p = {};
+    p.x = d->x, p.ldx = d->ldx, p.x16 = d->x_dtype == SWCB200_BF16;
+    p.residual = d->residual, p.ldr = d->ld_residual, p.r16 = d->residual_dtype == SWCB200_BF16;
+    p.gate = d->gate, p.ldg = d->ld_gate, p.g16 = d->gate_dtype == SWCB200_BF16;
+    p.sum = d->sum, p.lds = d->ld_sum, p.s16 = d->sum_dtype == SWCB200_BF16;
+    p.y = d->y, p.ldy = d->ldy, p.y16 = d->y_dtype == SWCB200_BF16;
+    p.rows = (long long)rows, p.gate_rows = d->gate_rows;
+    p.cols = cols, p.scale = d->scale, p.inv_cols = 1.0f / (float)cols;
+    p.post = {d->post.weight, d->post.bias, d->post.eps, d->post.kind};
+    p.pre = {d->pre.weight, d->pre.bias, d->pre.eps, d->pre.kind};
+
+    // chunks of 8: every row of every tensor starts on 16 bytes (bf16) or 32 (fp32), every vector on 16
+    bool vec = cols % 8 == 0;
+    const auto rows_ok = [&](const void *q, size_t ld, int is16, bool many) {
+        if (q) vec = vec && ((uintptr_t)q & (is16 ? 15u : 31u)) == 0 && (!many || ld % 8 == 0);
+    };
+    rows_ok(p.x, p.ldx, p.x16, rows > 1);
+    rows_ok(p.residual, p.ldr, p.r16, rows > 1);
+    rows_ok(p.sum, p.lds, p.s16, rows > 1);
+    rows_ok(p.y, p.ldy, p.y16, rows > 1);
+    rows_ok(p.gate, p.ldg, p.g16, p.gate_rows != 0);
+    for (const float *v : {p.post.w, p.post.b, p.pre.w, p.pre.b}) vec = vec && swc_aligned16(v);
+    const int chunks = vec ? cols / 8 : cols;
+    const int most = vec ? 4 : 32;  // chunks per thread: 32 elements
+    if (chunks <= 32 * most) {      // rows inside a warp
+        p.tpr = 1;
+        while (p.tpr < 32 && p.tpr * (vec ? 1 : 8) < chunks) p.tpr *= 2;
+        const int per_cta = 128 / p.tpr;
+        const unsigned grid = (unsigned)((rows + per_cta - 1) / per_cta);
+        const int n = (chunks + p.tpr - 1) / p.tpr;
+        vec ? launch<8, false>(n, grid, 128, ctx->stream, p) : launch<1, false>(n, grid, 128, ctx->stream, p);
+    } else {
+        int threads = (chunks + most - 1) / most;
+        threads = (threads + 31) / 32 * 32;
+        p.tpr = threads;
+        const int n = (chunks + threads - 1) / threads;
+        vec ? launch<8, true>(n, (unsigned)rows, threads, ctx->stream, p) : launch<1, true>(n, (unsigned)rows, threads, ctx->stream, p);
+    }
+    return swc_check_launch(ctx, "norm_residual");
+}

@@ -36,6 +36,23 @@ def pool_out_dims(idims, kernels, strides, pads):
             (w + pads[1] + pads[3] - kernels[1]) // strides[1] + 1, c)
 
 
+class _Norm(C.Structure):
+    _fields_ = [("kind", C.c_int), ("weight", C.c_void_p), ("bias", C.c_void_p), ("eps", C.c_float)]
+
+
+class _NormBlock(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_dtype", C.c_int), ("ldx", C.c_size_t), ("post", _Norm), ("gate", C.c_void_p),
+                ("gate_dtype", C.c_int), ("ld_gate", C.c_size_t), ("gate_rows", C.c_longlong), ("scale", C.c_float),
+                ("residual", C.c_void_p), ("residual_dtype", C.c_int), ("ld_residual", C.c_size_t), ("sum", C.c_void_p),
+                ("sum_dtype", C.c_int), ("ld_sum", C.c_size_t), ("pre", _Norm), ("y", C.c_void_p), ("y_dtype", C.c_int),
+                ("ldy", C.c_size_t)]
+
+
+class _FcEpilogue(C.Structure):
+    _fields_ = [("bias", C.c_void_p), ("act", C.c_int), ("scale", C.c_float), ("residual", C.c_void_p),
+                ("residual_dtype", C.c_int), ("ld_residual", C.c_int)]
+
+
 class Backend:
     def __init__(self, device: int | torch.device = 0, precision: int = L.STRICT_F32, own_stream: bool = False,
                  stream: "torch.cuda.Stream | None" = None):
@@ -107,6 +124,35 @@ class Backend:
                 continue
             if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
                 raise ValueError("expected a contiguous fp32 CUDA tensor")
+
+    def _on_device(self, what, *ts):
+        for t in ts:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{what}: expected a tensor on {self.device}, got one on {t.device}")
+
+    def _rows(self, what, *ts):
+        """[rows, cols] tensors, fp32 or bf16, each row contiguous, at any row pitch."""
+        self._on_device(what, *ts)
+        for t in ts:
+            if t is None:
+                continue
+            if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError(f"{what}: expected a 2-D fp32 or bf16 tensor")
+            if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+                raise ValueError(f"{what}: expected contiguous rows that do not overlap, got strides {t.stride()}")
+
+    def _vector(self, what, t, n):
+        self._on_device(what, t)
+        if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{what}: expected a contiguous fp32 tensor of {n} elements")
+
+    @staticmethod
+    def _ld(t):
+        return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    @staticmethod
+    def _dt(t):
+        return L.F32 if t is None or t.dtype == torch.float32 else L.BF16
 
     def _new(self, shape, dtype=torch.float32):
         return torch.empty(tuple(int(s) for s in shape), dtype=dtype, device=self.device)
@@ -327,3 +373,65 @@ class Backend:
         self._call("maxpool_bf16", _p(x), _p(out), _dims(x.shape), _dims(odims), _dims(kernels), _dims(strides),
                    _dims(pads))
         return out
+
+    # ---- transformer blocks -----------------------------------------------------
+    def fc_bf16_residual(self, a, wp, bias=None, act=L.ACT_NONE, residual=None, scale=1.0, out_dtype=torch.bfloat16, out=None):
+        """residual + scale * act(A[m,k] . Wp[n,k]^T + bias) in one launch.  A, Wp bf16, rows at any pitch that is a multiple
+        of 8; bias fp32 [n]; residual and `out` [m, n] fp32 or bf16, which may be one tensor.  All six activations."""
+        self._rows("fc_bf16_residual", a, wp, residual, out)
+        if a.dtype != torch.bfloat16 or wp.dtype != torch.bfloat16:
+            raise ValueError("fc_bf16_residual wants bf16 operands")
+        (m, k), (n, k2) = a.shape, wp.shape
+        if k != k2:
+            raise ValueError("inner dimensions differ")
+        self._vector("fc_bf16_residual", bias, n)
+        out = out if out is not None else self._new((m, n), out_dtype)
+        if out.shape != (m, n) or (residual is not None and residual.shape != (m, n)):
+            raise ValueError("fc_bf16_residual: residual and out are [m, n]")
+        ep = _FcEpilogue(bias.data_ptr() if bias is not None else None, act, scale,
+                         residual.data_ptr() if residual is not None else None, self._dt(residual), self._ld(residual))
+        pitch = lambda t: -(-t.shape[1] // 8) * 8 if t.shape[0] <= 1 else t.stride(0)  # one row has no pitch of its own
+        self._call("fc_bf16_residual", C.c_int(m), C.c_int(n), C.c_int(k), _p(a), C.c_int(pitch(a)), _p(wp), C.c_int(pitch(wp)),
+                   C.byref(ep), _p(out), C.c_int(self._dt(out)), C.c_int(self._ld(out)))
+        return out
+
+    def norm_residual(self, x, residual=None, post=None, gate=None, gate_rows=0, scale=1.0, pre=None, sum_dtype=None,
+                      y_dtype=torch.bfloat16, sum=None, y=None, want_sum=True):
+        """What lies between two blocks, in one launch: t = residual + scale * gate * post(x), y = pre(t).
+
+        x, residual [rows, cols] and gate [gates, cols] fp32 or bf16, rows at any pitch.  post and pre are norms
+        (kind, weight, bias, eps) with kind NORM_RMS or NORM_LAYER, weight and bias fp32 [cols] or None.  Gate row
+        r // gate_rows multiplies row r (gate_rows 0: one gate row for all).  Returns (t, y); t is None without
+        want_sum, y without pre.  `sum` (t's tensor) and `y` may be x or residual, which are then overwritten."""
+        self._rows("norm_residual", x, residual, gate, sum, y)
+        rows, cols = x.shape
+        if gate_rows < 0:
+            raise ValueError("norm_residual: negative gate_rows")
+        if gate is not None and (gate.shape[1] != cols or gate.shape[0] < (-(-rows // gate_rows) if gate_rows else 1)):
+            raise ValueError("norm_residual: too few gate rows, or of another width")
+        block = _NormBlock()
+        for name, n in (("post", post), ("pre", pre)):
+            if n is not None:
+                kind, weight, bias, eps = n
+                self._vector("norm_residual", weight, cols)
+                self._vector("norm_residual", bias, cols)
+                setattr(block, name, _Norm(kind, weight.data_ptr() if weight is not None else None,
+                                           bias.data_ptr() if bias is not None else None, eps))
+        if pre is None and y is not None:
+            raise ValueError("norm_residual: y goes with the norm that writes it")
+        if want_sum and sum is None:
+            sum = self._new((rows, cols), sum_dtype or (residual if residual is not None else x).dtype)
+        if pre is not None and y is None:
+            y = self._new((rows, cols), y_dtype)
+        for t in (residual, sum, y):
+            if t is not None and t.shape != x.shape:
+                raise ValueError("norm_residual: tensors of different shapes")
+        block.x, block.x_dtype, block.ldx = x.data_ptr(), self._dt(x), self._ld(x)
+        block.gate_rows, block.scale = gate_rows, scale
+        for name, ld, t in (("gate", "ld_gate", gate), ("residual", "ld_residual", residual), ("sum", "ld_sum", sum), ("y", "ldy", y)):
+            if t is not None:
+                setattr(block, name, t.data_ptr())
+            setattr(block, name + "_dtype", self._dt(t))
+            setattr(block, ld, self._ld(t))
+        self._call("norm_residual", C.c_size_t(rows), C.c_int(cols), C.byref(block))
+        return sum, y
