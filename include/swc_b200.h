@@ -300,6 +300,37 @@ typedef struct swcb200_norm_block {
 } swcb200_norm_block;
 int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, const swcb200_norm_block *block);
 
+/* Attention over packed sequences, one pass over the keys (running maximum and sum of the softmax):
+ *     o[i,h] = sum_j softmax_j(scale * q[i,h] . k[j,h']) v[j,h'],   h' = h / (heads_q / heads_kv)
+ * q, o [total_q, heads_q, head_dim], k, v [total_k, heads_kv, head_dim], bf16, at any row and head
+ * strides (elements); head_dim a multiple of 8 up to 128.  Sequence b owns rows q_offsets[b] ..
+ * q_offsets[b+1] of q and k_offsets[b] .. k_offsets[b+1] of k and v, or only the first k_lens[b] of
+ * these (a cache of fixed capacity); the arrays are int32 in DEVICE memory and are read by the
+ * kernels, so lengths may change between replays of a captured call.  causal: query i of n_q sees
+ * keys j <= i + n_k - n_q, else all.  A row that sees nothing gets o = 0 and lse = -infinity; rows
+ * of no sequence keep what they held.  Keys and values that no sequence owns may hold anything;
+ * within a sequence a value row that is not finite also reaches rows that the causal mask keeps
+ * from it.  Scores, softmax and sums are fp32 (the weights are rounded to bf16 for the second
+ * product).  Offsets are clamped to the tensors.  Alignment (TMA): bases on 16 bytes, strides
+ * multiples of 8.  o may not overlap q, k or v.  The workspace belongs to the call until it has
+ * finished on the stream: calls in flight together (two captured graphs, too) need one each. */
+typedef struct swcb200_attention {
+    const void *q, *k, *v;
+    void *o;
+    float *lse; /* [total_q, heads_q] log of the softmax's sum, or NULL */
+    size_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
+    int batch, total_q, total_k, heads_q, heads_kv, head_dim;
+    const int *q_offsets, *k_offsets; /* [batch + 1] */
+    const int *k_lens;                /* [batch] or NULL */
+    float scale;                      /* > 0 */
+    int causal;
+    void *workspace; /* 16-byte aligned; may be NULL where swcb200_attention_workspace says 0 */
+    size_t workspace_bytes;
+} swcb200_attention;
+/* Bytes that the call needs; reads batch, the totals, heads and head_dim only. */
+int swcb200_attention_workspace(swcb200_ctx *ctx, const swcb200_attention *a, size_t *bytes);
+int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention *a);
+
 /* ---------------------------------------------------- partitioned graphs
  * NCCL over NVLink in place of the MPI text ParallelCodegen prints
  * (src/codegen/ParallelCodegen.cpp:457-896).  One process per GPU.  `axis` follows the

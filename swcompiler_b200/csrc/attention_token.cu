@@ -1,0 +1,425 @@
+// Attention of a few new tokens per sequence over long caches.  What bounds it is reading the keys and values once.
+//
+// Rows of a tile are (token, head) pairs of the heads that read one key head, 16, 32 or 64 of them, so the cache is read once
+// for the whole group.  Work items are pieces of `part` keys of one sequence and key head (sequences of very different lengths
+// make items of the same size); persistent CTAs take them in turn, and a producer warp runs ahead over the items, so the ring of
+// 64-key blocks never drains between them.  Partial results of a sequence with several items go to the workspace and are joined
+// by a second kernel, in a fixed order; a sequence of one item is written directly.
+//
+// With 16 rows the tensor cores are a side matter (a 128-row tcgen05 tile would be seven eighths padding), so each warp runs
+// mma.sync m16n8k16 on 16 of a block's 64 keys with a softmax of its own in registers -- no barrier between warps until the end
+// of an item, where the four key groups are merged.
+#include "attention_common.cuh"
+
+namespace {
+
+using namespace tc;
+using namespace attn;
+
+constexpr int kKeys = 64;             // keys per block
+constexpr int kChunk = kKeys * 128;   // bytes of a 64-wide chunk of a block
+
+template <int CH, int RG> struct Shape {
+    static constexpr int kStage = 2 * CH * kChunk;  // K and V of a block
+    static constexpr int kStages = CH == 1 ? 8 : RG < 4 ? 5 : 4;
+    static constexpr int kPitch = CH * 64 + 8;      // of a row that is being merged: 16-byte rows, spread over the banks
+    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256 + (size_t)RG * 2 * 16 * kPitch * 4;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// items of a sequence for one unit of heads: pieces of its keys where its rows fit one tile, else its row tiles
+__device__ __forceinline__ int row_tiles(const Params &p, const Seq &s) { return (s.nq + p.tokens - 1) / p.tokens; }
+__device__ __forceinline__ int items_of(const Params &p, const Seq &s) {
+    const int rt = row_tiles(p, s);
+    return rt == 1 ? max((s.nk + p.part - 1) / p.part, 1) : rt;
+}
+
+struct Item {
+    Seq seq;
+    int index;     // over all sequences
+    int t0;        // first token of the rows
+    int k0, k1;    // keys
+    int unit;
+    bool partial;  // one of several pieces of its rows
+};
+
+__device__ __forceinline__ bool find_item(const Params &p, int work, Item &it) {
+    int i;
+    it.index = work / p.units;
+    it.unit = work - it.index * p.units;
+    if (it.index >= p.max_items || !find_seq(p, it.index, [&](const Seq &s) { return items_of(p, s); }, it.seq, i)) return false;
+    if (row_tiles(p, it.seq) == 1) {
+        it.t0 = 0;
+        it.k0 = i * p.part;
+        it.partial = it.seq.nk > p.part;
+    } else {
+        it.t0 = i * p.tokens;
+        it.k0 = 0;
+        it.partial = false;
+    }
+    const int sees = visible(p, it.seq, min(it.t0 + p.tokens, it.seq.nq) - 1);  // the last row sees the most
+    it.k1 = it.partial ? min(it.k0 + p.part, sees) : sees;
+    return true;
+}
+
+// RG groups of 16 rows x 4 groups of 16 keys of each block, a warp each, and a producer warp
+template <int CH, int RG>
+__global__ void __launch_bounds__(RG * 128 + 32, 1)
+attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p) {
+    using Sh = Shape<CH, RG>;
+    constexpr int kStages = Sh::kStages, kStage = Sh::kStage, kPitch = Sh::kPitch, kWarps = RG * 4, kD = CH * 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStage);
+    uint64_t *empty = full + kStages;
+    // merging: two slots per row group, 16 rows of kD outputs, then the maximum and the sum
+    float *merge = reinterpret_cast<float *>(smem + kStages * kStage + 256);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+        for (int s = 0; s < kStages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], kWarps);
+        }
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    __syncthreads();
+
+    int st = 0;
+    uint32_t ph = 0;
+    const auto next = [&] {
+        if (++st == kStages) {
+            st = 0;
+            ph ^= 1;
+        }
+    };
+    bool ok = true;
+    Item it;
+    if (warp == kWarps) {
+        // ------------------------------------------------------------ loads
+        for (int work = blockIdx.x; ok && find_item(p, work, it); work += gridDim.x) {
+            const int head_k = it.unit * p.pack / p.group;
+            for (int k = it.k0; k < it.k1 && ok; k += kKeys) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, p.status, kWaitEmpty));
+                if (!ok) break;
+                if (lane == 0) {
+                    uint8_t *dst = smem + st * kStage;
+                    mbar_expect_tx(&full[st], kStage);
+                    for (int c = 0; c < CH; c++) tma_load_3d(dst + c * kChunk, &tmK, &full[st], c * 64, head_k, it.seq.k0 + k);
+                    for (int c = 0; c < CH; c++) tma_load_3d(dst + (CH + c) * kChunk, &tmV, &full[st], c * 64, head_k, it.seq.k0 + k);
+                }
+                __syncwarp();
+                next();
+            }
+        }
+    } else {
+        const int rg = warp >> 2, kg = warp & 3;
+        const int g = lane >> 2, c2 = (lane & 3) * 2;  // row (and row + 8) and first column of this lane in mma fragments
+        // ldmatrix addresses inside a chunk: keys kg*16 + (0..15); the 16-byte piece is xor-ed with the row by the swizzle
+        const int k_row = kg * 16 + (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;   // K: (keys 0-7: d 0-7, 8-15), (keys 8-15: ..)
+        const int v_row = kg * 16 + (lane & 15), v_piece = lane >> 4;                            // V: (keys 0-7, 8-15: d 0-7), (.. d 8-15)
+        for (int work = blockIdx.x; ok && find_item(p, work, it); work += gridDim.x) {
+            // query fragments, rows g and g + 8 of this row group
+            uint32_t qf[kD / 16][4];
+            int sees[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = rg * 16 + g + h * 8, tok = row / p.pack, t = it.t0 + tok;
+                const bool valid = tok < p.tokens && t < it.seq.nq;
+                sees[h] = valid ? visible(p, it.seq, t) : 0;
+                const __nv_bfloat16 *src = p.q + (size_t)(it.seq.q0 + t) * p.q_row + (size_t)(it.unit * p.pack + row - tok * p.pack) * p.q_head;
+#pragma unroll
+                for (int s = 0; s < kD / 16; s++) {
+                    qf[s][h] = valid && s * 16 + c2 < p.d ? *reinterpret_cast<const uint32_t *>(src + s * 16 + c2) : 0u;
+                    qf[s][h + 2] = valid && s * 16 + c2 + 8 < p.d ? *reinterpret_cast<const uint32_t *>(src + s * 16 + c2 + 8) : 0u;
+                }
+            }
+            float o[kD / 8][4];
+#pragma unroll
+            for (int i = 0; i < kD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+            for (int k = it.k0; k < it.k1; k += kKeys) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&full[st], ph, p.status, kWaitFull));
+                if (!ok) break;
+                const uint32_t sk = smem_u32(smem + st * kStage), sv = sk + CH * kChunk;
+                const int first = k + kg * 16;  // this warp's first key
+                if (first < it.k1) {
+                    float s[2][4] = {};
+#pragma unroll
+                    for (int i = 0; i < kD / 16; i++) {
+                        uint32_t b[4];
+                        const int piece = (i & 3) * 2 + k_piece;
+                        ldmatrix4(b, sk + (i >> 2) * kChunk + k_row * 128 + ((piece ^ (k_row & 7)) << 4));
+                        mma_16x8x16(s[0], qf[i][0], qf[i][1], qf[i][2], qf[i][3], b[0], b[1]);
+                        mma_16x8x16(s[1], qf[i][0], qf[i][1], qf[i][2], qf[i][3], b[2], b[3]);
+                    }
+                    uint32_t w[4];  // the weights as the A operand of the second product
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float x[4] = {s[0][2 * h], s[0][2 * h + 1], s[1][2 * h], s[1][2 * h + 1]};
+                        const int lim = min(sees[h], it.k1) - first - c2;
+                        x[0] = lim > 0 ? x[0] : -INFINITY;
+                        x[1] = lim > 1 ? x[1] : -INFINITY;
+                        x[2] = lim > 8 ? x[2] : -INFINITY;
+                        x[3] = lim > 9 ? x[3] : -INFINITY;
+                        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        float factor = 1.f;
+                        if ((mx - m[h]) * p.scale_log2 > kSlack) {  // also where m is -inf; not where mx is (NaN compares false)
+                            factor = exp2_fast((m[h] - mx) * p.scale_log2);
+                            m[h] = mx;
+                        }
+                        if (__any_sync(0xffffffffu, factor != 1.f)) {
+                            l[h] *= factor;
+#pragma unroll
+                            for (int i = 0; i < kD / 8; i++) {
+                                o[i][2 * h] *= factor;
+                                o[i][2 * h + 1] *= factor;
+                            }
+                        }
+                        const float base = m[h] == -INFINITY ? 0.f : m[h] * p.scale_log2;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[i] = exp2_fast(fmaf(x[i], p.scale_log2, -base));
+                        l[h] += (x[0] + x[1]) + (x[2] + x[3]);
+                        w[h] = pack_bf16(x[0], x[1]);
+                        w[h + 2] = pack_bf16(x[2], x[3]);
+                    }
+                    // Keys past the item's last one have weight 0, but their V belongs to somebody else (or to nobody), and 0 times
+                    // infinity or NaN is not 0: those rows of V count as 0.
+                    const int lim = it.k1 - first - c2;
+                    const uint32_t keep0 = lim > 1 ? 0xffffffffu : lim > 0 ? 0x0000ffffu : 0u;
+                    const uint32_t keep1 = lim > 9 ? 0xffffffffu : lim > 8 ? 0x0000ffffu : 0u;
+                    const bool whole = first + 16 <= it.k1;
+#pragma unroll
+                    for (int i = 0; i < kD / 16; i++) {
+                        uint32_t b[4];
+                        const int piece = (i & 3) * 2 + v_piece;
+                        ldmatrix4_trans(b, sv + (i >> 2) * kChunk + v_row * 128 + ((piece ^ (v_row & 7)) << 4));
+                        if (!whole) {
+                            b[0] &= keep0;
+                            b[1] &= keep1;
+                            b[2] &= keep0;
+                            b[3] &= keep1;
+                        }
+                        mma_16x8x16(o[2 * i], w[0], w[1], w[2], w[3], b[0], b[1]);
+                        mma_16x8x16(o[2 * i + 1], w[0], w[1], w[2], w[3], b[2], b[3]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[st]);
+                next();
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            }
+            // merge the four key groups: 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+            for (int step = 2; step >= 1; step >>= 1) {
+                if (kg >= step && kg < 2 * step) {
+                    float *dst = merge + (rg * 2 + kg - step) * 16 * kPitch;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float *r = dst + (g + 8 * h) * kPitch;
+#pragma unroll
+                        for (int i = 0; i < kD / 8; i++) *reinterpret_cast<float2 *>(r + i * 8 + c2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+                        if (c2 == 0) *reinterpret_cast<float2 *>(r + kD) = make_float2(m[h], l[h]);
+                    }
+                }
+                named_barrier(1 + rg, 128);
+                if (kg < step) {
+                    const float *src = merge + (rg * 2 + kg) * 16 * kPitch;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float *r = src + (g + 8 * h) * kPitch;
+                        const float2 ml = *reinterpret_cast<const float2 *>(r + kD);
+                        const float top = fmaxf(m[h], ml.x);
+                        const float a = m[h] == -INFINITY ? 0.f : exp2_fast((m[h] - top) * p.scale_log2);
+                        const float b = ml.x == -INFINITY ? 0.f : exp2_fast((ml.x - top) * p.scale_log2);
+                        // (a group without keys has l = 0 and o = 0, or NaN where its scores were NaN: kept by the plain sums below)
+                        l[h] = l[h] * (m[h] == -INFINITY ? 1.f : a) + ml.y * (ml.x == -INFINITY ? 1.f : b);
+#pragma unroll
+                        for (int i = 0; i < kD / 8; i++) {
+                            const float2 v = *reinterpret_cast<const float2 *>(r + i * 8 + c2);
+                            o[i][2 * h] = o[i][2 * h] * a + v.x * b;
+                            o[i][2 * h + 1] = o[i][2 * h + 1] * a + v.y * b;
+                        }
+                        m[h] = top;
+                    }
+                }
+                named_barrier(1 + rg, 128);
+            }
+            if (kg == 0) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int row = rg * 16 + g + h * 8, tok = row / p.pack, t = it.t0 + tok;
+                    if (tok >= p.tokens || t >= it.seq.nq) continue;
+                    const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+                    const int head = it.unit * p.pack + row - tok * p.pack;
+                    if (it.partial) {
+                        const size_t slot = ((size_t)it.index * p.units + it.unit) * (RG * 16) + row;
+                        float *dst = p.part_o + slot * p.d;
+#pragma unroll
+                        for (int i = 0; i < kD / 8; i++)
+                            if (i * 8 < p.d) *reinterpret_cast<float2 *>(dst + i * 8 + c2) = make_float2(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
+                        if (c2 == 0) p.part_lse[slot] = l[h] == 0.f ? -INFINITY : fmaf(m[h], p.scale_log2, log2f(l[h]));
+                    } else {
+                        const size_t at = (size_t)(it.seq.q0 + t);
+                        __nv_bfloat16 *dst = p.o + at * p.o_row + (size_t)head * p.o_head;
+#pragma unroll
+                        for (int i = 0; i < kD / 8; i++)
+                            if (i * 8 < p.d) *reinterpret_cast<uint32_t *>(dst + i * 8 + c2) = pack_bf16(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
+                        if (c2 == 0 && p.lse)
+                            p.lse[at * p.heads_q + head] =
+                                l[h] == 0.f ? -INFINITY : 0.69314718055994531f * fmaf(m[h], p.scale_log2, log2f(l[h]));
+                    }
+                }
+            }
+        }
+    }
+    // a wait that gave up leaves copies possibly still in flight towards this CTA's shared memory: a bounded time to land
+    if (!ok) {
+        const long long since = clock64();
+        while (clock64() - since < 4000000ll) {
+        }
+    }
+    __syncwarp();
+}
+
+// Joins the parts of a row: a CTA per (token, head), warps take parts in turn, then a fixed-order sum over the warps.
+// kItems: parts are the items of the token kernel (slot = item), else `parts` of every token of the prompt kernel.
+constexpr int kJoinWarps = 8;
+template <bool kItems>
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const Params p, int rows, int parts) {
+    __shared__ float s_o[kJoinWarps][128], s_l[kJoinWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int token = blockIdx.x / p.heads_q, head = blockIdx.x - token * p.heads_q;
+    size_t slot, step;
+    int n;
+    if (kItems) {
+        // the sequence that holds the token, and the items before it
+        int before = 0, found = -1;
+        Seq seq = {0, 0, 0, 0};
+        for (int base = 0; base < p.batch && found < 0; base += 32) {
+            Seq s = {0, 0, 0, 0};
+            int count = 0;
+            if (base + lane < p.batch) {
+                s = load_seq(p, base + lane);
+                count = items_of(p, s);
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, token >= s.q0 && token < s.q0 + s.nq);
+            const int src = hit ? __ffs(hit) - 1 : 32;
+            int add = lane < src ? count : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+            before += add;
+            if (hit) {
+                found = base + src;
+                seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+                seq.nq = __shfl_sync(0xffffffffu, s.nq, src);
+                seq.nk = __shfl_sync(0xffffffffu, s.nk, src);
+            }
+        }
+        if (found < 0 || row_tiles(p, seq) != 1 || seq.nk <= p.part) return;  // no sequence's row, or written already
+        n = min(items_of(p, seq), p.max_items - before);
+        const int unit = head / p.pack;
+        slot = ((size_t)before * p.units + unit) * rows + (token - seq.q0) * p.pack + (head - unit * p.pack);
+        step = (size_t)p.units * rows;
+    } else {
+        bool mine = false;  // rows of no sequence stay as they were
+        for (int b = lane; b < p.batch; b += 32) {
+            const Seq s = load_seq(p, b);
+            mine = mine || (token >= s.q0 && token < s.q0 + s.nq);
+        }
+        if (!__any_sync(0xffffffffu, mine)) return;
+        n = parts;
+        slot = (size_t)token * p.heads_q + head;
+        step = (size_t)p.total_q * p.heads_q;
+    }
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_lse[slot + i * step]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    const int c = lane * 4;
+#pragma unroll 4
+    for (int i = warp; i < n; i += kJoinWarps) {
+        const size_t at = slot + i * step;
+        const float w = exp2_fast(p.part_lse[at] - base);
+        l += w;
+        if (c < p.d) {
+            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at * p.d + c);
+            acc[0] = fmaf(w, v.x, acc[0]);
+            acc[1] = fmaf(w, v.y, acc[1]);
+            acc[2] = fmaf(w, v.z, acc[2]);
+            acc[3] = fmaf(w, v.w, acc[3]);
+        }
+    }
+    *reinterpret_cast<float4 *>(&s_o[warp][c]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    const int d = threadIdx.x;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) sum += s_l[w];
+    if (d < p.d) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; w++) v += s_o[w][d];
+        p.o[(size_t)token * p.o_row + (size_t)head * p.o_head + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
+    }
+    if (d == 0 && p.lse) p.lse[(size_t)token * p.heads_q + head] = sum == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(sum));
+}
+
+template <int CH, int RG>
+int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmK, const CUtensorMap &tmV, int max_items) {
+    const size_t smem = Shape<CH, RG>::kSmem;
+    SWC_CUDA(ctx, cudaFuncSetAttribute(attention_token_kernel<CH, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const long long work = (long long)max_items * p.units;
+    const unsigned grid = (unsigned)(work < ctx->sm_count ? work : ctx->sm_count);
+    attention_token_kernel<CH, RG><<<grid, RG * 128 + 32, smem, ctx->stream>>>(tmK, tmV, p);
+    return swc_check_launch(ctx, "attention_bf16");
+}
+
+}  // namespace
+
+int swc_attention_token(swcb200_ctx *ctx, Params &p, const CUtensorMap &tmK, const CUtensorMap &tmV, int rows, int max_items) {
+    int rc;
+    if (p.d > 64)
+        rc = rows == 16 ? launch<2, 1>(ctx, p, tmK, tmV, max_items) : rows == 32 ? launch<2, 2>(ctx, p, tmK, tmV, max_items) : launch<2, 4>(ctx, p, tmK, tmV, max_items);
+    else
+        rc = rows == 16 ? launch<1, 1>(ctx, p, tmK, tmV, max_items) : rows == 32 ? launch<1, 2>(ctx, p, tmK, tmV, max_items) : launch<1, 4>(ctx, p, tmK, tmV, max_items);
+    if (rc || p.part >= p.total_k) return rc;  // no sequence has more than one part
+    attention_join_kernel<true><<<(unsigned)p.total_q * p.heads_q, kJoinWarps * 32, 0, ctx->stream>>>(p, rows, 0);
+    return swc_check_launch(ctx, "attention_bf16");
+}
+
+int swc_attention_join_parts(swcb200_ctx *ctx, Params &p, int parts) {
+    attention_join_kernel<false><<<(unsigned)p.total_q * p.heads_q, kJoinWarps * 32, 0, ctx->stream>>>(p, 0, parts);
+    return swc_check_launch(ctx, "attention_bf16");
+}

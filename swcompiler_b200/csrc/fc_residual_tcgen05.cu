@@ -117,6 +117,19 @@ __device__ __forceinline__ void drain_after_failure() {
     }
 }
 
+// tokens t .. t + kTok - 1 of this CTA's `own`: their partial sums added in rank order
+template <int kTok>
+__device__ __forceinline__ void finish_joined(const FcrParams &p, const float *slots, int own, int t, int row, int token, int col,
+                                              float bias) {
+    float v[kTok];
+#pragma unroll
+    for (int j = 0; j < kTok; j++) v[j] = 0.f;
+    for (int s = 0; s < p.splits; s++)
+#pragma unroll
+        for (int j = 0; j < kTok; j++) v[j] += slots[(s * own + t + j) * BM + row];
+    finish<kTok>(p, v, token, col, bias);
+}
+
 constexpr int kSplitThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
 
 // shared memory: `stages` x (weight tile, token tile), then the join's slots [splits][BN / splits][128] fp32, then barriers
@@ -228,17 +241,21 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
                 }
             } else {
                 // this CTA's partial sums go to the CTAs that own the tokens, slot `rank`
-                const int own = p.bn / p.splits;
+                const int own = p.bn / p.splits;  // a power of two, at least 2
+                const int own_log2 = 31 - __clz(own);
+                const uint32_t mine = smem_u32(slots + (int)rank * own * BM + row);
                 for (int c0 = 0; c0 < p.bn; c0 += 16) {
                     if (tm * p.bn + c0 >= p.m) break;
                     uint32_t r[16];
                     tmem_ld_32x16(taddr + c0, r);
                     tmem_ld_wait();
+                    // 16 columns lie in one owner's part (own >= 16) or cover 16 / own owners
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int q = (c0 + j) / own, t = (c0 + j) - q * own;
-                        if (tm * p.bn + c0 + j < p.m)
-                            st_cluster(map_to_cta(smem_u32(slots + ((int)rank * own + t) * BM + row), (uint32_t)q), __uint_as_float(r[j]));
+                    for (int j = 0; j < 16; j += 2) {
+                        const int q = (c0 + j) >> own_log2, t = (c0 + j) & (own - 1);
+                        const uint32_t dst = map_to_cta(mine + (uint32_t)t * (BM * 4), (uint32_t)q);
+                        st_cluster(dst, __uint_as_float(r[j]));
+                        st_cluster(dst + BM * 4, __uint_as_float(r[j + 1]));
                     }
                 }
             }
@@ -254,12 +271,11 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
             const int row = (warp & 3) * 32 + lane, col = tn * BM + row;
             const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
             const int own = p.bn / p.splits;
-            for (int t = 0; t < own; t++) {
-                const int token = tm * p.bn + (int)rank * own + t;
-                if (token >= p.m) break;
-                float v[1] = {0.f};
-                for (int s = 0; s < p.splits; s++) v[0] += slots[(s * own + t) * BM + row];
-                finish<1>(p, v, token, col, bias);
+            const int token0 = tm * p.bn + (int)rank * own;
+            if (own < 8) {
+                for (int t = 0; t < own; t += 2) finish_joined<2>(p, slots, own, t, row, token0 + t, col, bias);
+            } else {
+                for (int t = 0; t < own; t += 8) finish_joined<8>(p, slots, own, t, row, token0 + t, col, bias);
             }
         }
     }

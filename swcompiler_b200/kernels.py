@@ -48,6 +48,14 @@ class _NormBlock(C.Structure):
                 ("ldy", C.c_size_t)]
 
 
+class _Attention(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "o", "lse")] +
+                [(n, C.c_size_t) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head")] +
+                [(n, C.c_int) for n in ("batch", "total_q", "total_k", "heads_q", "heads_kv", "head_dim")] +
+                [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_lens")] +
+                [("scale", C.c_float), ("causal", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)])
+
+
 class _FcEpilogue(C.Structure):
     _fields_ = [("bias", C.c_void_p), ("act", C.c_int), ("scale", C.c_float), ("residual", C.c_void_p),
                 ("residual_dtype", C.c_int), ("ld_residual", C.c_int)]
@@ -109,6 +117,11 @@ class Backend:
     def selftest_wait_timeout(self):
         """Launches a kernel whose bounded wait can only run out; `sync()` then raises with status ERR_TIMEOUT."""
         self._call("selftest_wait_timeout")
+
+    def _issue_stream(self):
+        if self.torch_stream is None:
+            return torch.cuda.ExternalStream(self.lib.swcb200_stream(self._ctx), self.device)
+        return self.torch_stream
 
     def set_precision(self, precision: int):
         self._call("set_precision", C.c_int(precision))
@@ -435,3 +448,37 @@ class Backend:
             setattr(block, ld, self._ld(t))
         self._call("norm_residual", C.c_size_t(rows), C.c_int(cols), C.byref(block))
         return sum, y
+
+    def attention_bf16(self, q, k, v, q_offsets, k_offsets, k_lens=None, scale=None, causal=True, out=None, lse=None):
+        """softmax(scale * q . k^T) . v over packed sequences.  q [total_q, heads_q, d], k, v [total_k, heads_kv, d] bf16 at any
+        row and head strides (multiples of 8), d a multiple of 8 up to 128; q_offsets, k_offsets int32 [batch + 1] on the
+        device; k_lens int32 [batch]: only that many of a sequence's key rows are filled.  scale: d ** -0.5 unless given.
+        causal: query i of n_q sees keys j <= i + n_k - n_q.  `lse` fp32 [total_q, heads_q] receives the log of each softmax's
+        sum.  Rows of `out` that belong to no sequence keep what they held."""
+        self._on_device("attention_bf16", q, k, v, q_offsets, k_offsets, k_lens, out, lse)
+        for t in (q, k, v, out):
+            if t is not None and (t.dim() != 3 or t.dtype != torch.bfloat16 or (t.numel() and t.shape[2] > 1 and t.stride(2) != 1)):
+                raise ValueError("attention_bf16: q, k, v and out are bf16 [rows, heads, d] with contiguous d")
+        (tq, hq, d), (tk, hkv, dk) = q.shape, k.shape
+        if v.shape != k.shape or dk != d or (out is not None and out.shape != q.shape):
+            raise ValueError("attention_bf16: q, out [total_q, heads_q, d] and k, v [total_k, heads_kv, d]")
+        batch = q_offsets.numel() - 1
+        for t, n in ((q_offsets, batch + 1), (k_offsets, batch + 1), (k_lens, batch)):
+            if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.numel() != n or batch < 0):
+                raise ValueError("attention_bf16: offsets are contiguous int32 [batch + 1], k_lens [batch]")
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tq, hq) or not lse.is_contiguous()):
+            raise ValueError("attention_bf16: lse is a contiguous fp32 tensor [total_q, heads_q]")
+        out = out if out is not None else self._new(q.shape, torch.bfloat16)
+        a = _Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+                       q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1),
+                       batch, tq, tk, hq, hkv, d, q_offsets.data_ptr(), k_offsets.data_ptr(),
+                       k_lens.data_ptr() if k_lens is not None else None, d ** -0.5 if scale is None else scale, int(causal))
+        need = C.c_size_t()
+        self._call("attention_workspace", C.byref(a), C.byref(need))
+        if need.value:
+            # from the memory pool of the stream that the kernels run on: handed out again only to work behind them
+            with torch.cuda.stream(self._issue_stream()):
+                ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+        self._call("attention_bf16", C.byref(a))
+        return out
