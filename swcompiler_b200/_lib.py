@@ -48,6 +48,12 @@ def lib() -> C.CDLL:
         l.swcb200_stream.argtypes = [C.c_void_p]
         l.swcb200_launch_count.restype = C.c_uint64
         l.swcb200_launch_count.argtypes = [C.c_void_p]
+        # the calls that pass plain integers and packed structs
+        i, z, p, b = C.c_int, C.c_size_t, C.c_void_p, C.c_char_p
+        l.swcb200_fc_bf16_residual.argtypes = [p, i, i, i, p, i, p, i, b, p, i, i]
+        l.swcb200_norm_residual.argtypes = [p, z, i, b]
+        l.swcb200_attention_workspace.argtypes = [p, b, C.POINTER(z)]
+        l.swcb200_attention_bf16.argtypes = [p, b]
         _lib = l
     return _lib
 

@@ -9,6 +9,7 @@ library.  torch is used for device memory and streams, nothing else.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -36,29 +37,11 @@ def pool_out_dims(idims, kernels, strides, pads):
             (w + pads[1] + pads[3] - kernels[1]) // strides[1] + 1, c)
 
 
-class _Norm(C.Structure):
-    _fields_ = [("kind", C.c_int), ("weight", C.c_void_p), ("bias", C.c_void_p), ("eps", C.c_float)]
-
-
-class _NormBlock(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("x_dtype", C.c_int), ("ldx", C.c_size_t), ("post", _Norm), ("gate", C.c_void_p),
-                ("gate_dtype", C.c_int), ("ld_gate", C.c_size_t), ("gate_rows", C.c_longlong), ("scale", C.c_float),
-                ("residual", C.c_void_p), ("residual_dtype", C.c_int), ("ld_residual", C.c_size_t), ("sum", C.c_void_p),
-                ("sum_dtype", C.c_int), ("ld_sum", C.c_size_t), ("pre", _Norm), ("y", C.c_void_p), ("y_dtype", C.c_int),
-                ("ldy", C.c_size_t)]
-
-
-class _Attention(C.Structure):
-    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "o", "lse")] +
-                [(n, C.c_size_t) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head")] +
-                [(n, C.c_int) for n in ("batch", "total_q", "total_k", "heads_q", "heads_kv", "head_dim")] +
-                [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_lens")] +
-                [("scale", C.c_float), ("causal", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)])
-
-
-class _FcEpilogue(C.Structure):
-    _fields_ = [("bias", C.c_void_p), ("act", C.c_int), ("scale", C.c_float), ("residual", C.c_void_p),
-                ("residual_dtype", C.c_int), ("ld_residual", C.c_int)]
+# layouts of the header's structs, packed in one call (native alignment; a test compares them with the compiler's)
+_FC_EPILOGUE = struct.Struct("@PifPii")
+_NORM_BLOCK = struct.Struct("@PiN" "iPPf4x" "PiNqf" "PiN" "PiN" "iPPf4x" "PiN")
+_ATTENTION = struct.Struct("@5P8N6i3PfiPN")
+_DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
 class Backend:
@@ -70,6 +53,7 @@ class Backend:
             raise RuntimeError("swcompiler_b200 needs a CUDA device; there is no CPU path")
         self.lib = L.lib()
         self.device = torch.device("cuda", device if isinstance(device, int) else device.index or 0)
+        self._index = self.device.index
         self._ctx = C.c_void_p()
         self.torch_stream = None
         with torch.cuda.device(self.device):
@@ -138,34 +122,26 @@ class Backend:
             if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
                 raise ValueError("expected a contiguous fp32 CUDA tensor")
 
-    def _on_device(self, what, *ts):
-        for t in ts:
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{what}: expected a tensor on {self.device}, got one on {t.device}")
-
-    def _rows(self, what, *ts):
-        """[rows, cols] tensors, fp32 or bf16, each row contiguous, at any row pitch."""
-        self._on_device(what, *ts)
-        for t in ts:
-            if t is None:
-                continue
-            if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16):
-                raise ValueError(f"{what}: expected a 2-D fp32 or bf16 tensor")
-            if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
-                raise ValueError(f"{what}: expected contiguous rows that do not overlap, got strides {t.stride()}")
+    def _matrix(self, what, t):
+        """(address, dtype, leading dimension, rows, columns) of an fp32 or bf16 matrix with contiguous rows at any pitch."""
+        dtype = _DTYPES.get(t.dtype)
+        if dtype is None or t.ndim != 2 or t.get_device() != self._index:
+            raise ValueError(f"{what}: expected an fp32 or bf16 matrix on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        rows, cols = t.shape
+        pitch, step = t.stride()
+        if rows <= 1:
+            pitch = cols
+        if (step != 1 and cols > 1 or pitch < cols) and rows:
+            raise ValueError(f"{what}: expected contiguous rows that do not overlap, got strides {t.stride()}")
+        return t.data_ptr(), dtype, pitch, rows, cols
 
     def _vector(self, what, t, n):
-        self._on_device(what, t)
-        if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
-            raise ValueError(f"{what}: expected a contiguous fp32 tensor of {n} elements")
-
-    @staticmethod
-    def _ld(t):
-        return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-    @staticmethod
-    def _dt(t):
-        return L.F32 if t is None or t.dtype == torch.float32 else L.BF16
+        """Address of an fp32 vector of n elements; 0 for None."""
+        if t is None:
+            return 0
+        if t.dtype != torch.float32 or t.ndim != 1 or t.numel() != n or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{what}: expected a contiguous fp32 vector of {n} elements on {self.device}")
+        return t.data_ptr()
 
     def _new(self, shape, dtype=torch.float32):
         return torch.empty(tuple(int(s) for s in shape), dtype=dtype, device=self.device)
@@ -391,21 +367,33 @@ class Backend:
     def fc_bf16_residual(self, a, wp, bias=None, act=L.ACT_NONE, residual=None, scale=1.0, out_dtype=torch.bfloat16, out=None):
         """residual + scale * act(A[m,k] . Wp[n,k]^T + bias) in one launch.  A, Wp bf16, rows at any pitch that is a multiple
         of 8; bias fp32 [n]; residual and `out` [m, n] fp32 or bf16, which may be one tensor.  All six activations."""
-        self._rows("fc_bf16_residual", a, wp, residual, out)
-        if a.dtype != torch.bfloat16 or wp.dtype != torch.bfloat16:
+        what = "fc_bf16_residual"
+        pa, ta, lda, m, k = self._matrix(what, a)
+        pw, tw, ldw, n, k2 = self._matrix(what, wp)
+        if ta != L.BF16 or tw != L.BF16:
             raise ValueError("fc_bf16_residual wants bf16 operands")
-        (m, k), (n, k2) = a.shape, wp.shape
         if k != k2:
             raise ValueError("inner dimensions differ")
-        self._vector("fc_bf16_residual", bias, n)
-        out = out if out is not None else self._new((m, n), out_dtype)
-        if out.shape != (m, n) or (residual is not None and residual.shape != (m, n)):
-            raise ValueError("fc_bf16_residual: residual and out are [m, n]")
-        ep = _FcEpilogue(bias.data_ptr() if bias is not None else None, act, scale,
-                         residual.data_ptr() if residual is not None else None, self._dt(residual), self._ld(residual))
-        pitch = lambda t: -(-t.shape[1] // 8) * 8 if t.shape[0] <= 1 else t.stride(0)  # one row has no pitch of its own
-        self._call("fc_bf16_residual", C.c_int(m), C.c_int(n), C.c_int(k), _p(a), C.c_int(pitch(a)), _p(wp), C.c_int(pitch(wp)),
-                   C.byref(ep), _p(out), C.c_int(self._dt(out)), C.c_int(self._ld(out)))
+        if m <= 1:
+            lda = (k + 7) & ~7  # one row has no pitch of its own
+        if n <= 1:
+            ldw = (k + 7) & ~7
+        pr, tr, ldr = 0, 0, 0
+        if residual is not None:
+            pr, tr, ldr, rows, cols = self._matrix(what, residual)
+            if rows != m or cols != n:
+                raise ValueError("fc_bf16_residual: residual and out are [m, n]")
+        if out is None:
+            out = torch.empty(m, n, dtype=out_dtype, device=self.device)
+            pc, tc, ldc = out.data_ptr(), _DTYPES[out_dtype], n
+        else:
+            pc, tc, ldc, rows, cols = self._matrix(what, out)
+            if rows != m or cols != n:
+                raise ValueError("fc_bf16_residual: residual and out are [m, n]")
+        rc = self.lib.swcb200_fc_bf16_residual(self._ctx, m, n, k, pa, lda, pw, ldw,
+                                               _FC_EPILOGUE.pack(self._vector(what, bias, n), act, scale, pr, tr, ldr), pc, tc, ldc)
+        if rc:
+            self._check(rc, what)
         return out
 
     def norm_residual(self, x, residual=None, post=None, gate=None, gate_rows=0, scale=1.0, pre=None, sum_dtype=None,
@@ -416,37 +404,48 @@ class Backend:
         (kind, weight, bias, eps) with kind NORM_RMS or NORM_LAYER, weight and bias fp32 [cols] or None.  Gate row
         r // gate_rows multiplies row r (gate_rows 0: one gate row for all).  Returns (t, y); t is None without
         want_sum, y without pre.  `sum` (t's tensor) and `y` may be x or residual, which are then overwritten."""
-        self._rows("norm_residual", x, residual, gate, sum, y)
-        rows, cols = x.shape
-        if gate_rows < 0:
-            raise ValueError("norm_residual: negative gate_rows")
-        if gate is not None and (gate.shape[1] != cols or gate.shape[0] < (-(-rows // gate_rows) if gate_rows else 1)):
-            raise ValueError("norm_residual: too few gate rows, or of another width")
-        block = _NormBlock()
-        for name, n in (("post", post), ("pre", pre)):
-            if n is not None:
-                kind, weight, bias, eps = n
-                self._vector("norm_residual", weight, cols)
-                self._vector("norm_residual", bias, cols)
-                setattr(block, name, _Norm(kind, weight.data_ptr() if weight is not None else None,
-                                           bias.data_ptr() if bias is not None else None, eps))
-        if pre is None and y is not None:
-            raise ValueError("norm_residual: y goes with the norm that writes it")
-        if want_sum and sum is None:
-            sum = self._new((rows, cols), sum_dtype or (residual if residual is not None else x).dtype)
-        if pre is not None and y is None:
-            y = self._new((rows, cols), y_dtype)
-        for t in (residual, sum, y):
-            if t is not None and t.shape != x.shape:
+        what = "norm_residual"
+        px, tx, ldx, rows, cols = self._matrix(what, x)
+        p_res = p_sum = p_y = p_gate = t_res = t_sum = t_y = t_gate = ld_res = ld_sum = ld_y = ld_gate = 0
+        if residual is not None:
+            p_res, t_res, ld_res, r, c = self._matrix(what, residual)
+            if r != rows or c != cols:
                 raise ValueError("norm_residual: tensors of different shapes")
-        block.x, block.x_dtype, block.ldx = x.data_ptr(), self._dt(x), self._ld(x)
-        block.gate_rows, block.scale = gate_rows, scale
-        for name, ld, t in (("gate", "ld_gate", gate), ("residual", "ld_residual", residual), ("sum", "ld_sum", sum), ("y", "ldy", y)):
-            if t is not None:
-                setattr(block, name, t.data_ptr())
-            setattr(block, name + "_dtype", self._dt(t))
-            setattr(block, ld, self._ld(t))
-        self._call("norm_residual", C.c_size_t(rows), C.c_int(cols), C.byref(block))
+        if gate is not None:
+            p_gate, t_gate, ld_gate, r, c = self._matrix(what, gate)
+            if gate_rows < 0 or c != cols or r < (-(-rows // gate_rows) if gate_rows else 1):
+                raise ValueError("norm_residual: too few gate rows, or of another width")
+        k_post = w_post = b_post = e_post = k_pre = w_pre = b_pre = e_pre = 0
+        if post is not None:
+            k_post, weight, bias, e_post = post
+            w_post, b_post = self._vector(what, weight, cols), self._vector(what, bias, cols)
+        if pre is not None:
+            k_pre, weight, bias, e_pre = pre
+            w_pre, b_pre = self._vector(what, weight, cols), self._vector(what, bias, cols)
+        elif y is not None:
+            raise ValueError("norm_residual: y goes with the norm that writes it")
+        if sum is None:
+            if want_sum:
+                sum_dtype = sum_dtype or (x if residual is None else residual).dtype
+                sum = torch.empty(rows, cols, dtype=sum_dtype, device=self.device)
+                p_sum, t_sum, ld_sum = sum.data_ptr(), _DTYPES[sum_dtype], cols
+        else:
+            p_sum, t_sum, ld_sum, r, c = self._matrix(what, sum)
+            if r != rows or c != cols:
+                raise ValueError("norm_residual: tensors of different shapes")
+        if y is not None:
+            p_y, t_y, ld_y, r, c = self._matrix(what, y)
+            if r != rows or c != cols:
+                raise ValueError("norm_residual: tensors of different shapes")
+        elif pre is not None:
+            y = torch.empty(rows, cols, dtype=y_dtype, device=self.device)
+            p_y, t_y, ld_y = y.data_ptr(), _DTYPES[y_dtype], cols
+        rc = self.lib.swcb200_norm_residual(
+            self._ctx, rows, cols,
+            _NORM_BLOCK.pack(px, tx, ldx, k_post, w_post, b_post, e_post, p_gate, t_gate, ld_gate, gate_rows, scale, p_res, t_res,
+                             ld_res, p_sum, t_sum, ld_sum, k_pre, w_pre, b_pre, e_pre, p_y, t_y, ld_y))
+        if rc:
+            self._check(rc, what)
         return sum, y
 
     def attention_bf16(self, q, k, v, q_offsets, k_offsets, k_lens=None, scale=None, causal=True, out=None, lse=None):
@@ -455,30 +454,58 @@ class Backend:
         device; k_lens int32 [batch]: only that many of a sequence's key rows are filled.  scale: d ** -0.5 unless given.
         causal: query i of n_q sees keys j <= i + n_k - n_q.  `lse` fp32 [total_q, heads_q] receives the log of each softmax's
         sum.  Rows of `out` that belong to no sequence keep what they held."""
-        self._on_device("attention_bf16", q, k, v, q_offsets, k_offsets, k_lens, out, lse)
-        for t in (q, k, v, out):
-            if t is not None and (t.dim() != 3 or t.dtype != torch.bfloat16 or (t.numel() and t.shape[2] > 1 and t.stride(2) != 1)):
-                raise ValueError("attention_bf16: q, k, v and out are bf16 [rows, heads, d] with contiguous d")
-        (tq, hq, d), (tk, hkv, dk) = q.shape, k.shape
-        if v.shape != k.shape or dk != d or (out is not None and out.shape != q.shape):
+        what = "attention_bf16"
+        pq, tq, hq, d, q_row, q_head = self._heads(what, q)
+        pk, tk, hkv, dk, k_row, k_head = self._heads(what, k)
+        pv, tv, hv, dv, v_row, v_head = self._heads(what, v)
+        if out is None:
+            out = torch.empty(tq, hq, d, dtype=torch.bfloat16, device=self.device)
+            po, o_row, o_head, fits = out.data_ptr(), hq * d, d, True
+        else:
+            po, to, ho, do, o_row, o_head = self._heads(what, out)
+            fits = to == tq and ho == hq and do == d
+        if tv != tk or hv != hkv or dv != d or dk != d or not fits:
             raise ValueError("attention_bf16: q, out [total_q, heads_q, d] and k, v [total_k, heads_kv, d]")
         batch = q_offsets.numel() - 1
-        for t, n in ((q_offsets, batch + 1), (k_offsets, batch + 1), (k_lens, batch)):
-            if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.numel() != n or batch < 0):
-                raise ValueError("attention_bf16: offsets are contiguous int32 [batch + 1], k_lens [batch]")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tq, hq) or not lse.is_contiguous()):
-            raise ValueError("attention_bf16: lse is a contiguous fp32 tensor [total_q, heads_q]")
-        out = out if out is not None else self._new(q.shape, torch.bfloat16)
-        a = _Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
-                       q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1),
-                       batch, tq, tk, hq, hkv, d, q_offsets.data_ptr(), k_offsets.data_ptr(),
-                       k_lens.data_ptr() if k_lens is not None else None, d ** -0.5 if scale is None else scale, int(causal))
+        p_qo, p_ko = self._lengths(what, q_offsets, batch + 1), self._lengths(what, k_offsets, batch + 1)
+        p_kl = 0 if k_lens is None else self._lengths(what, k_lens, batch)
+        p_lse = 0
+        if lse is not None:
+            if lse.dtype != torch.float32 or lse.shape != (tq, hq) or not lse.is_contiguous() or lse.get_device() != self._index:
+                raise ValueError("attention_bf16: lse is a contiguous fp32 tensor [total_q, heads_q]")
+            p_lse = lse.data_ptr()
+        call = (pq, pk, pv, po, p_lse, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, batch, tq, tk, hq, hkv, d,
+                p_qo, p_ko, p_kl, d ** -0.5 if scale is None else scale, 1 if causal else 0)
         need = C.c_size_t()
-        self._call("attention_workspace", C.byref(a), C.byref(need))
+        rc = self.lib.swcb200_attention_workspace(self._ctx, _ATTENTION.pack(*call, 0, 0), C.byref(need))
+        if rc:
+            self._check(rc, what)
+        p_ws = 0
         if need.value:
             # from the memory pool of the stream that the kernels run on: handed out again only to work behind them
-            with torch.cuda.stream(self._issue_stream()):
+            stream = self._issue_stream()
+            if stream == torch.cuda.current_stream(self.device):
                 ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-        self._call("attention_bf16", C.byref(a))
+            else:
+                with torch.cuda.stream(stream):
+                    ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+            p_ws = ws.data_ptr()
+        rc = self.lib.swcb200_attention_bf16(self._ctx, _ATTENTION.pack(*call, p_ws, need.value))
+        if rc:
+            self._check(rc, what)
         return out
+
+    def _heads(self, what, t):
+        """(address, rows, heads, width, row stride, head stride) of a bf16 tensor [rows, heads, width] with contiguous widths."""
+        if t.dtype != torch.bfloat16 or t.ndim != 3 or t.get_device() != self._index:
+            raise ValueError(f"{what}: expected bf16 [rows, heads, d] on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        rows, heads, d = t.shape
+        row, head, step = t.stride()
+        if step != 1 and d > 1:
+            raise ValueError(f"{what}: the last dimension of {tuple(t.shape)} is not contiguous")
+        return t.data_ptr(), rows, heads, d, row, head
+
+    def _lengths(self, what, t, n):
+        if t.dtype != torch.int32 or t.ndim != 1 or t.numel() != n or n < 0 or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{what}: offsets are contiguous int32 [batch + 1] and k_lens int32 [batch], on {self.device}")
+        return t.data_ptr()
