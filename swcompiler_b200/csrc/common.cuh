@@ -69,6 +69,32 @@ static inline int swc_tc_sms(const swcb200_ctx *ctx) {
 
 static inline bool swc_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Launch of a kernel that may start while the stream's previous kernel still runs: it sets itself up, then waits with
+// swc_after_previous() before it touches anything the previous kernel wrote.  A kernel that has called swc_let_next_start() in
+// all of its blocks lets such a successor take the SMs' free resources at once.
+template <class... P, class... A>
+static inline cudaError_t swc_launch_early(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
+                                           unsigned cluster, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ void swc_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void swc_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+
 // Grid for a grid-stride kernel: enough CTAs to cover `work_items` at `per_cta`, capped at a
 // whole number of waves over the SMs.
 static inline unsigned swc_grid(const swcb200_ctx *ctx, size_t work_items, size_t per_cta, int ctas_per_sm) {

@@ -105,8 +105,8 @@ __device__ __forceinline__ void finish(const FcrParams &p, const float (&acc)[kT
     }
 }
 
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // A wait that gave up leaves copies possibly still in flight towards this CTA's shared memory: give them a bounded time to land
@@ -117,29 +117,34 @@ __device__ __forceinline__ void drain_after_failure() {
     }
 }
 
-// tokens t .. t + kTok - 1 of this CTA's `own`: their partial sums added in rank order
+// kTok tokens of one column: the partial sums of all slots added in rank order
 template <int kTok>
-__device__ __forceinline__ void finish_joined(const FcrParams &p, const float *slots, int own, int t, int row, int token, int col,
-                                              float bias) {
+__device__ __forceinline__ void finish_joined(const FcrParams &p, const float *mine, int slot, int token, int col, float bias) {
     float v[kTok];
 #pragma unroll
     for (int j = 0; j < kTok; j++) v[j] = 0.f;
     for (int s = 0; s < p.splits; s++)
 #pragma unroll
-        for (int j = 0; j < kTok; j++) v[j] += slots[(s * own + t + j) * BM + row];
+        for (int j = 0; j < kTok; j++) v[j] += mine[s * slot + j * BM];
     finish<kTok>(p, v, token, col, bias);
 }
 
 constexpr int kSplitThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
 
-// shared memory: `stages` x (weight tile, token tile), then the join's slots [splits][BN / splits][128] fp32, then barriers
+// shared memory: `stages` x (weight tile, token tile), then barriers; once every CTA of the cluster has multiplied its last stage
+// the ring becomes the join's slots, [splits][own][128 rows] fp32 with own = BN / splits tokens: a warp's store to another CTA is
+// 128 contiguous bytes (16-byte pieces at the pitch of a row took 2 us longer per join)
+// kSub: 64-deep blocks per stage of the ring.  Two of them halve the waits and commits, which at few tokens cost the issuing
+// threads more than the blocks do (64 tokens, 4096 x 4096, k undivided: 22.1 -> 17.7 us); at 256 tokens a stage of one keeps the
+// ring four deep.
+template <int kSub>
 __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                      const __grid_constant__ CUtensorMap tmA, const FcrParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t stage_bytes = W_BYTES + (uint32_t)p.bn * BK * 2;
-    float *slots = reinterpret_cast<float *>(smem + (size_t)p.stages * stage_bytes);
-    uint64_t *full = reinterpret_cast<uint64_t *>(slots + (p.splits > 1 ? p.bn * BM : 0));
+    const uint32_t block_bytes = W_BYTES + (uint32_t)p.bn * BK * 2, stage_bytes = kSub * block_bytes;
+    float *slots = reinterpret_cast<float *>(smem);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + (size_t)p.stages * stage_bytes);
     uint64_t *empty = full + p.stages;
     uint64_t *done = empty + p.stages;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(done + 1);
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     const uint32_t rank = p.splits > 1 ? cluster_ctarank() : 0;
     const int tile = blockIdx.x / p.splits;
     const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
-    const int kblocks = (p.k + BK - 1) / BK;
+    const int kblocks = (p.k + kSub * BK - 1) / (kSub * BK);
     const int kb0 = (int)((long long)kblocks * rank / p.splits), kb1 = (int)((long long)kblocks * (rank + 1) / p.splits);
 
     if (threadIdx.x == 0) {
@@ -169,10 +174,14 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     }
     tc_fence_before();
     __syncthreads();
-    if (p.splits > 1) cluster_sync();  // every CTA of the cluster runs before its shared memory is written from another
+    swc_let_next_start();
+    swc_after_previous();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
     bool failed = false;
+    // epilogue warps: a row of the tile (an output column) per thread, in the lane quarter that the warp may read
+    const int row = (warp & 3) * 32 + lane, col = tn * BM + row;
+    const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -185,8 +194,11 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
                 }
                 mbar_expect_tx(&full[st], stage_bytes);
                 uint8_t *sw = smem + (size_t)st * stage_bytes;
-                tma_load_2d(sw, &tmW, &full[st], kb * BK, tn * BM);
-                tma_load_2d(sw + W_BYTES, &tmA, &full[st], kb * BK, tm * p.bn);
+#pragma unroll
+                for (int b = 0; b < kSub; b++) {
+                    tma_load_2d(sw + b * block_bytes, &tmW, &full[st], (kb * kSub + b) * BK, tn * BM);
+                    tma_load_2d(sw + b * block_bytes + W_BYTES, &tmA, &full[st], (kb * kSub + b) * BK, tm * p.bn);
+                }
                 if (++st == p.stages) {
                     st = 0;
                     ph ^= 1;
@@ -205,10 +217,13 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
                 }
                 tc_fence_after();
                 const uint32_t sw = smem_u32(smem + (size_t)st * stage_bytes);
-                const uint64_t dw = smem_desc_sw128(sw), da = smem_desc_sw128(sw + W_BYTES);
 #pragma unroll
-                for (int j = 0; j < BK / UMMA_K; j++)
-                    umma_bf16(tmem_base, dw + 2 * j, da + 2 * j, idesc, (uint32_t)(kb != kb0 || j != 0));
+                for (int b = 0; b < kSub; b++) {
+                    const uint64_t dw = smem_desc_sw128(sw + b * block_bytes), da = smem_desc_sw128(sw + b * block_bytes + W_BYTES);
+#pragma unroll
+                    for (int j = 0; j < BK / UMMA_K; j++)
+                        umma_bf16(tmem_base, dw + 2 * j, da + 2 * j, idesc, (uint32_t)(kb != kb0 || b + j != 0));
+                }
                 umma_commit(&empty[st]);
                 if (++st == p.stages) {
                     st = 0;
@@ -222,42 +237,18 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
         if (lane == 0) ok = mbar_wait(done, 0, p.status, kWaitTmemFull);
         failed = !__shfl_sync(0xffffffffu, ok, 0);
         tc_fence_after();
-        const int quarter = warp & 3, row = quarter * 32 + lane;
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        const int col = tn * BM + row;
-        if (!failed) {
-            if (p.splits == 1) {
-                const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
-                for (int c0 = 0; c0 < p.bn; c0 += 16) {
-                    if (tm * p.bn + c0 >= p.m) break;
-                    uint32_t r[16];
-                    float acc[16];
-                    tmem_ld_32x16(taddr + c0, r);
-                    tmem_ld_wait();
+        if (!failed && p.splits == 1) {
+            const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
+            for (int c0 = 0; c0 < p.bn; c0 += 16) {
+                if (tm * p.bn + c0 >= p.m) break;
+                uint32_t r[16];
+                float acc[16];
+                tmem_ld_32x16(taddr + c0, r);
+                tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) acc[j] = __uint_as_float(r[j]);
-                    finish<16>(p, acc, tm * p.bn + c0, col, bias);
-                    __syncwarp();
-                }
-            } else {
-                // this CTA's partial sums go to the CTAs that own the tokens, slot `rank`
-                const int own = p.bn / p.splits;  // a power of two, at least 2
-                const int own_log2 = 31 - __clz(own);
-                const uint32_t mine = smem_u32(slots + (int)rank * own * BM + row);
-                for (int c0 = 0; c0 < p.bn; c0 += 16) {
-                    if (tm * p.bn + c0 >= p.m) break;
-                    uint32_t r[16];
-                    tmem_ld_32x16(taddr + c0, r);
-                    tmem_ld_wait();
-                    // 16 columns lie in one owner's part (own >= 16) or cover 16 / own owners
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const int q = (c0 + j) >> own_log2, t = (c0 + j) & (own - 1);
-                        const uint32_t dst = map_to_cta(mine + (uint32_t)t * (BM * 4), (uint32_t)q);
-                        st_cluster(dst, __uint_as_float(r[j]));
-                        st_cluster(dst + BM * 4, __uint_as_float(r[j + 1]));
-                    }
-                }
+                for (int j = 0; j < 16; j++) acc[j] = __uint_as_float(r[j]);
+                finish<16>(p, acc, tm * p.bn + c0, col, bias);
+                __syncwarp();
             }
         }
     }
@@ -266,23 +257,133 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     if (p.splits > 1) {
+        cluster_sync();  // every CTA has read its last stage: the rings may be overwritten
+        const int own = p.bn / p.splits, own_log2 = 31 - __clz(own);  // a power of two, at least 2
+        if (warp >= 2) {
+            // this CTA's partial sums go to the CTAs that own the tokens, slot `rank`
+            tc_fence_after();
+            const uint32_t mine = smem_u32(slots + (int)rank * own * BM + row);
+            for (int c0 = 0; c0 < p.bn; c0 += 16) {
+                if (tm * p.bn + c0 >= p.m) break;
+                uint32_t r[16];
+                tmem_ld_32x16(taddr + c0, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const int q = (c0 + j) >> own_log2, t = (c0 + j) & (own - 1);
+                    const uint32_t dst = map_to_cta(mine + (uint32_t)t * (BM * 4), (uint32_t)q);
+                    st_cluster(dst, r[j]);
+                    st_cluster(dst + BM * 4, r[j + 1]);
+                }
+            }
+        }
         cluster_sync();  // all partial sums have arrived
         if (warp >= 2) {
-            const int row = (warp & 3) * 32 + lane, col = tn * BM + row;
             const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
-            const int own = p.bn / p.splits;
-            const int token0 = tm * p.bn + (int)rank * own;
-            if (own < 8) {
-                for (int t = 0; t < own; t += 2) finish_joined<2>(p, slots, own, t, row, token0 + t, col, bias);
-            } else {
-                for (int t = 0; t < own; t += 8) finish_joined<8>(p, slots, own, t, row, token0 + t, col, bias);
-            }
+            const float *mine = slots + row;
+            const int token0 = tm * p.bn + (int)rank * own, slot = own * BM;
+            if (own == 2)
+                finish_joined<2>(p, mine, slot, token0, col, bias);
+            else if (own < 16)
+                for (int t = 0; t < own; t += 4) finish_joined<4>(p, mine + t * BM, slot, token0 + t, col, bias);
+            else
+                for (int t = 0; t < own; t += 16) finish_joined<16>(p, mine + t * BM, slot, token0 + t, col, bias);
         }
     }
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem_base, tmem_cols);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Up to four tokens.  Reading the weights is all there is to it (a multiply-add per weight and token), and at these sizes a call is
+// a few microseconds, of which a tensor-core kernel's set-up and drain would be half: here every thread requests its whole share of
+// 8 (4 tokens: 4) weight rows at once, multiplies on the FP32 pipe, and the CTA adds up.
+constexpr int kFewThreads = 256;
+__host__ __device__ constexpr int few_rows(int tokens) { return tokens > 2 ? 4 : 8; }
+
+// sums of kV values over the 32 lanes: lane l ends up with the sum of value l % kV
+template <int kV> __device__ __forceinline__ float lanes_sum(float (&v)[kV], int lane) {
+#pragma unroll
+    for (int n = kV / 2; n >= 1; n /= 2) {  // halve the values: keep the half that this lane's bit names, send the other
+        const bool upper = lane & n;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+        }
+    }
+#pragma unroll
+    for (int o = kV; o < 32; o *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    return v[0];
+}
+
+// the last `count` < 8 elements of a row, zeros behind them
+__device__ __noinline__ uint4 load_end(const __nv_bfloat16 *p, int count) {
+    uint32_t r[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 7; e++)
+        if (e < count) r[e / 2] |= (uint32_t)__bfloat16_as_ushort(p[e]) << (e & 1) * 16;
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int kTokens>
+__global__ void __launch_bounds__(kFewThreads) fc_res_few_kernel(const __nv_bfloat16 *__restrict__ a, size_t lda,
+                                                                 const __nv_bfloat16 *__restrict__ w, size_t ldw, const FcrParams p) {
+    constexpr int kFewRows = few_rows(kTokens), kV = kFewRows * kTokens;
+    __shared__ float part[kFewThreads / 32][kV];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n0 = blockIdx.x * kFewRows;
+    float acc[kV];
+#pragma unroll
+    for (int i = 0; i < kV; i++) acc[i] = 0.f;
+    swc_let_next_start();
+    swc_after_previous();
+    // k in steps of 8 elements per thread
+#pragma unroll 2
+    for (int k = threadIdx.x * 8; k < p.k; k += kFewThreads * 8) {
+        uint4 wv[kFewRows], av[kTokens];
+        if (k + 8 <= p.k) {
+#pragma unroll
+            for (int r = 0; r < kFewRows; r++) {
+                const __nv_bfloat16 *src = w + (size_t)min(n0 + r, p.n - 1) * ldw + k;
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(wv[r].x), "=r"(wv[r].y), "=r"(wv[r].z), "=r"(wv[r].w)
+                             : "l"(src));
+            }
+#pragma unroll
+            for (int t = 0; t < kTokens; t++) av[t] = __ldg(reinterpret_cast<const uint4 *>(a + (size_t)min(t, p.m - 1) * lda + k));
+        } else {  // the end of the rows: nothing behind it is read
+#pragma unroll
+            for (int r = 0; r < kFewRows; r++) wv[r] = load_end(w + (size_t)min(n0 + r, p.n - 1) * ldw + k, p.k - k);
+#pragma unroll
+            for (int t = 0; t < kTokens; t++) av[t] = load_end(a + (size_t)min(t, p.m - 1) * lda + k, p.k - k);
+        }
+#pragma unroll
+        for (int t = 0; t < kTokens; t++) {
+            const uint32_t x[4] = {av[t].x, av[t].y, av[t].z, av[t].w};
+#pragma unroll
+            for (int r = 0; r < kFewRows; r++) {
+                const uint32_t y[4] = {wv[r].x, wv[r].y, wv[r].z, wv[r].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    acc[t * kFewRows + r] = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), acc[t * kFewRows + r]);
+                    acc[t * kFewRows + r] = fmaf(__uint_as_float(x[e] & 0xffff0000u), __uint_as_float(y[e] & 0xffff0000u), acc[t * kFewRows + r]);
+                }
+            }
+        }
+    }
+    const float sum = lanes_sum<kV>(acc, lane);
+    if (lane < kV) part[warp][lane] = sum;
+    __syncthreads();
+    if (threadIdx.x < kV) {
+        const int t = threadIdx.x / kFewRows, col = n0 + threadIdx.x % kFewRows;
+        float v[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < kFewThreads / 32; i++) v[0] += part[i][threadIdx.x];
+        if (col < p.n) finish<1>(p, v, t, col, p.bias ? __ldg(p.bias + col) : 0.f);
     }
 }
 
@@ -346,6 +447,8 @@ fc_res_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     tc_fence_before();
     __syncthreads();
     cluster_sync();  // the peer's barriers exist before anything is signalled across the pair
+    swc_let_next_start();
+    swc_after_previous();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
     bool failed = false;
@@ -462,8 +565,31 @@ int tmap_rows(swcb200_ctx *ctx, const void *base, int rows, int cols, int ld, in
     return make_tmap_bf16(ctx, out, base, 2, dims, strides, box);
 }
 
-size_t split_smem(const FcrParams &p) {
-    return (size_t)p.stages * (W_BYTES + p.bn * BK * 2) + (p.splits > 1 ? (size_t)p.bn * BM * 4 : 0) + 1024 + 256;
+constexpr int kSplitSmem = 226 * 1024;
+
+struct Choice {
+    bool pair;
+    int bn, splits;
+};
+
+// The form with the least time by a model of it: waves over the SMs, times what a CTA spends on its k blocks and beside them.
+// Measured at k = 4096, in us: a 64-deep block takes 0.11 / 0.12 / 0.155 / 0.19 / 0.28 at 16 / 32 / 64 / 128 / 256 tokens (the
+// issuing threads, then loads), 0.30 in the pair form (the tensor pipe at 256 x 256); launch, first loads, epilogue 6.5 + 0.016 per
+// token; the join over 2 / 4 / 8 CTAs 0.8 / 2 / 3.5.  (m, n) = (777, 1000): chosen 128 tokens over 2 CTAs 14.7 us; 4 CTAs (two
+// waves) 21.6; undivided 19.9; 256 tokens over 4 18.1; pairs 26.1.  (64, 4096): 64 over 4 11.1; over 8 12.4; undivided 17.7.
+Choice choose(int m, int n, int kblocks, int sms) {
+    Choice best = {true, BN_MAX, 1};
+    const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
+    double least = sms < 2 ? 1e30 : (double)up(up(n, 2 * BM) * up(m, BN_MAX), sms / 2) * kblocks * 0.30 + 6.5;
+    const double step[5] = {0.11, 0.12, 0.155, 0.19, 0.28}, join[4] = {0, 0.8, 2.0, 3.5};
+    for (int i = 0; i < 5; i++)
+        for (int j = 0; j < 4; j++) {
+            const int bn = 16 << i, s = 1 << j;
+            if ((j > 0 && s * 2 > kblocks) || (i > 0 && bn >= 2 * m)) continue;
+            const double t = (double)up(up(n, BM) * up(m, bn) * s, sms) * ((double)up(kblocks, s) * step[i] + 6.5 + 0.016 * bn + join[j]);
+            if (t < least) least = t, best = {false, bn, s};
+        }
+    return best;
 }
 
 }  // namespace
@@ -497,49 +623,46 @@ SWC_EXPORT int swcb200_fc_bf16_residual(swcb200_ctx *ctx, int m, int n, int k, c
     const int sms = swc_tc_sms(ctx);
     CUtensorMap tmW, tmA;
 
-    const long long pairs = sms / 2;
-    const long long tiles256 = (long long)((n + 255) / 256) * ((m + 255) / 256);
-    if (tiles256 >= pairs && pairs > 0) {
-        p.bn = BN_MAX;
+    if (m <= 4) {  // 8.3 us against 10.2 at one token, 4096 x 4096
+        const auto kernel = m == 1 ? fc_res_few_kernel<1> : m == 2 ? fc_res_few_kernel<2> : fc_res_few_kernel<4>;
+        SWC_CUDA(ctx, swc_launch_early(kernel, (unsigned)((n + few_rows(m) - 1) / few_rows(m)), kFewThreads, 0, ctx->stream, 1,
+                                       (const __nv_bfloat16 *)a_bf16, (size_t)lda, (const __nv_bfloat16 *)wp_bf16, (size_t)ldw, p));
+        return swc_check_launch(ctx, "fc_bf16_residual");
+    }
+    const int kblocks = (k + BK - 1) / BK;
+    const Choice best = choose(m, n, kblocks, sms);
+    p.bn = best.bn;
+    p.splits = best.splits;
+    p.tiles_m = (m + p.bn - 1) / p.bn;
+    if (best.pair) {
         p.tiles_n = (n + 2 * BM - 1) / (2 * BM);
-        p.tiles_m = (m + p.bn - 1) / p.bn;
         SWC_REQUIRE(ctx, (long long)p.tiles_n * p.tiles_m < 0x7fffffff, SWCB200_ERR_TOO_LARGE, "fc_bf16_residual: too many tiles");
         p.band = ((size_t)n * k * 2 <= ((size_t)48 << 20) || p.tiles_n <= 8) ? p.tiles_n : 8;
         int rc = tmap_rows(ctx, wp_bf16, n, k, ldw, BM, &tmW);
         if (!rc) rc = tmap_rows(ctx, a_bf16, m, k, lda, p.bn / 2, &tmA);
         if (rc) return rc;
         SWC_CUDA(ctx, cudaFuncSetAttribute(fc_res_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem));
-        const long long tiles = (long long)p.tiles_n * p.tiles_m;
-        const unsigned grid = 2u * (unsigned)(tiles < pairs ? tiles : pairs);
-        fc_res_pair_kernel<<<grid, kPairThreads, kPairSmem, ctx->stream>>>(tmW, tmA, p);
+        const long long tiles = (long long)p.tiles_n * p.tiles_m, pairs = sms / 2;
+        SWC_CUDA(ctx, swc_launch_early(fc_res_pair_kernel, 2u * (unsigned)(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem,
+                                       ctx->stream, 1, tmW, tmA, p));
         return swc_check_launch(ctx, "fc_bf16_residual");
     }
-    p.bn = 16;
-    while (p.bn < m && p.bn < 128) p.bn *= 2;
     p.tiles_n = (n + BM - 1) / BM;
-    p.tiles_m = (m + p.bn - 1) / p.bn;
     SWC_REQUIRE(ctx, (long long)p.tiles_n * p.tiles_m < 0x7fffffff / 8, SWCB200_ERR_TOO_LARGE, "fc_bf16_residual: too many tiles");
-    const long long tiles = (long long)p.tiles_n * p.tiles_m;
-    const int kblocks = (k + BK - 1) / BK;
-    p.splits = 1;
-    while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sms && kblocks >= p.splits * 2 * 4) p.splits *= 2;
-    p.stages = p.bn <= 32 ? 5 : 4;
+    // the ring: as deep as the CTA's k range and shared memory allow, and never smaller than the join's slots
+    const int sub = p.bn > 128 ? 1 : 2;
+    const int stage = sub * (W_BYTES + p.bn * BK * 2);
+    const int most = (kblocks + sub * p.splits - 1) / (sub * p.splits), fit = (kSplitSmem - 1280) / stage;
+    p.stages = most < fit ? most : fit;
+    const int slots = p.splits > 1 ? BM * p.bn * 4 : 0;
+    if (p.stages * stage < slots) p.stages = (slots + stage - 1) / stage;
     int rc = tmap_rows(ctx, wp_bf16, n, k, ldw, BM, &tmW);
     if (!rc) rc = tmap_rows(ctx, a_bf16, m, k, lda, p.bn, &tmA);
     if (rc) return rc;
-    const size_t smem = split_smem(p);
-    SWC_CUDA(ctx, cudaFuncSetAttribute(fc_res_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * p.splits));
-    cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)p.splits;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    SWC_CUDA(ctx, cudaLaunchKernelEx(&cfg, fc_res_split_kernel, tmW, tmA, p));
+    const size_t smem = (size_t)p.stages * stage + 1280;
+    const auto kernel = sub == 1 ? fc_res_split_kernel<1> : fc_res_split_kernel<2>;
+    SWC_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem));
+    SWC_CUDA(ctx, swc_launch_early(kernel, (unsigned)((long long)p.tiles_n * p.tiles_m * p.splits), kSplitThreads, smem, ctx->stream,
+                                   (unsigned)p.splits, tmW, tmA, p));
     return swc_check_launch(ctx, "fc_bf16_residual");
 }
