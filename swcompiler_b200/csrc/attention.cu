@@ -150,7 +150,7 @@ SWC_EXPORT int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention 
     p.q_off = a->q_offsets, p.k_off = a->k_offsets, p.k_lens = a->k_lens;
     p.batch = a->batch, p.total_q = a->total_q, p.total_k = a->total_k;
     p.heads_q = a->heads_q, p.group = a->heads_q / a->heads_kv, p.d = a->head_dim;
-    p.pack = pl.pack, p.units = pl.units, p.tokens = pl.tokens;
+    p.pack = pl.pack, p.pack_inv = (65536u + pl.pack - 1) / pl.pack, p.units = pl.units, p.tokens = pl.tokens;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.causal = a->causal != 0;
     p.part = pl.part, p.max_items = pl.max_items;
@@ -158,7 +158,7 @@ SWC_EXPORT int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention 
     p.part_lse = (float *)((char *)a->workspace + pl.lse_at);
     p.status = ctx->dev_status;
     CUtensorMap tmQ, tmK, tmV;
-    const int keys = pl.token ? 64 : 128;
+    const int keys = pl.token ? 64 : 128;  // of a block
     if ((rc = tmap_heads(ctx, k, a->head_dim, 1, keys, &tmK)) || (rc = tmap_heads(ctx, v, a->head_dim, 1, keys, &tmV))) return rc;
     if (pl.token) return swc_attention_token(ctx, p, tmK, tmV, pl.rows, pl.max_items);
     if ((rc = tmap_heads(ctx, q, a->head_dim, pl.pack, pl.tokens, &tmQ))) return rc;

@@ -14,6 +14,7 @@ struct Params {
     int batch, total_q, total_k;
     int heads_q, group, d;  // group: query heads per key head
     int pack;               // query heads in one tile (a divisor of group): tile rows are (token, head), head fastest
+    unsigned pack_inv;      // (2^16 + pack - 1) / pack: x / pack = x * pack_inv >> 16 for the rows x of a tile, 0 .. 127
     int units;              // heads_q / pack
     int tokens;             // tokens per tile
     float scale_log2;       // scale * log2(e): the softmax runs on powers of two
