@@ -49,34 +49,17 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The products' instructions are unrolled with constant offsets, and of a descriptor only the low word is computed: what the
-// issuing thread does between two of them is time that the tensor pipe idles (a loop over 64-bit descriptors took 130 to 160
-// cycles per instruction of 64).
-__device__ __forceinline__ void umma_scores(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-        "setp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-// D (+)= A[tmem] . B[smem]: the weights are the A operand in tensor memory
-__device__ __forceinline__ void umma_output(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool accumulate) {
+// D (+)= A[tmem] . B[smem]: the weights are the A operand in tensor memory; V is the B operand with its columns (d) contiguous, keys
+// as rows of 128 bytes, and the second chunk of 64 columns kChunk bytes behind the first (the leading offset of its descriptor)
+__device__ __forceinline__ void umma_output(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
         "setp.ne.b32 p, %5, 0;\n\t"
         "mov.b64 b, {%2, %3};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)accumulate)
+        "r"(a_tmem), "r"(b_lo), "r"(kDescHigh), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
-
-// Descriptor words.  High: 8 rows 1024 bytes apart, version 1, 128-byte swile.  Low: address, and the leading offset, which K-major
-// operands (Q, K) do not use; V is the B operand with its columns (d) contiguous, keys as rows of 128 bytes, and the second chunk of
-// 64 columns kChunk bytes behind the first.
-constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t leading) { return ((saddr & 0x3FFFF) >> 4) | (leading >> 4 << 16); }
 
 // Two fp32 at a time (one instruction for both)
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -137,11 +120,6 @@ __device__ __forceinline__ void load_masked(uint32_t t_s, int seen, float (&s)[3
     tmem_ld_wait();
 #pragma unroll
     for (int i = 0; i < 32; i++) s[i] = i < seen ? s[i] : -INFINITY;
-}
-
-// a whole warp waits, and gives up together
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int *status, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
 }
 
 // Takes over a block of the grid that has not started: 16 bytes of answer land at `result`, counted on `bar`.
@@ -412,7 +390,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
                     for (int s = 0; s < CH * 4; s++) {
                         const uint32_t off = (s >> 2) * (kChunk >> 4) + (s & 3) * 2;
-                        if (s < dk) umma_scores(tmem + h * kKeys, dq + off, dkey + off, kDescHigh, idesc_s, s != 0);
+                        if (s < dk) umma_bf16_words(tmem + h * kKeys, dq + off, dkey + off, idesc_s, s != 0);
                     }
                     umma_commit(&s_full[h]);
                     if (j + 1 == w.n(h)) umma_commit(&q_empty[h]);
@@ -461,7 +439,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         if (elect_one()) {
 #pragma unroll
                             for (int s = 0; s < kKeys / 32; s++)
-                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), kDescHigh, idesc_o, true);
+                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
                         }
                         __syncwarp();
                         if (stage_k < 0) stage_k = take_stage();
@@ -471,11 +449,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         if (!failed && elect_one()) {
 #pragma unroll
                             for (int s = kKeys / 32; s < kKeys / 16; s++)
-                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), kDescHigh, idesc_o, true);
+                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
 #pragma unroll
                             for (int s = 0; s < CH * 4; s++) {
                                 const uint32_t off = (s >> 2) * (kChunk >> 4) + (s & 3) * 2;
-                                umma_scores(t_s, q_lo + h * (kBlock >> 4) + off, dkey + off, kDescHigh, idesc_bf16_f32(kRows, kKeys), s != 0);
+                                umma_bf16_words(t_s, q_lo + h * (kBlock >> 4) + off, dkey + off, idesc_bf16_f32(kRows, kKeys), s != 0);
                             }
                             umma_commit(&s_full[h]);
                             if (j + 2 == now.n(h)) umma_commit(&q_empty[h]);
@@ -492,7 +470,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         if (!failed && elect_one()) {
 #pragma unroll
                             for (int s = 0; s < kKeys / 32; s++)
-                                if (s < steps) umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), kDescHigh, idesc_o, s != 0 || j != 0);
+                                if (s < steps) umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, s != 0 || j != 0);
                         }
                         __syncwarp();
                         wait(&p_full[h], parity, kWaitTmemEmpty);
@@ -500,7 +478,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         if (!failed && elect_one()) {
 #pragma unroll
                             for (int s = kKeys / 32; s < kKeys / 16; s++)
-                                if (s < steps) umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), kDescHigh, idesc_o, true);
+                                if (s < steps) umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
                             if (j + 1 == now.n(h)) umma_commit(&o_full[h]);
                         }
                         __syncwarp();

@@ -2,8 +2,9 @@
 //
 // Rows of a tile are (token, head) pairs of the heads that read one key head, 16, 32 or 64 of them, so the cache is read once
 // for the whole group.  Work items are pieces of `part` keys of one sequence and key head (sequences of very different lengths
-// make items of the same size); persistent CTAs take them in turn, and a producer warp runs ahead over the items, so the ring of
-// 64-key blocks never drains between them.  Partial results of a sequence with several items go to the workspace and are joined
+// make items of the same size); persistent CTAs take them in turn.  One warp finds the items and brings their query rows into
+// shared memory, another one loads their keys and values; both run ahead of the products, so the ring of 64-key blocks does not
+// drain between items.  Partial results of a sequence with several items go to the workspace and are joined
 // by a second kernel, in a fixed order; a sequence of one item is written directly.
 //
 // With 16 rows the tensor cores are a side matter (a 128-row tcgen05 tile would be seven eighths padding), so each warp runs
@@ -21,9 +22,11 @@ constexpr int kChunk = kKeys * 128;   // bytes of a 64-wide chunk of a block
 
 template <int CH, int RG> struct Shape {
     static constexpr int kStage = 2 * CH * kChunk;  // K and V of a block
-    static constexpr int kStages = CH == 1 ? 8 : RG < 4 ? 5 : 4;
+    static constexpr int kStages = CH == 1 ? 8 : RG < 4 ? 5 : 3;
     static constexpr int kPitch = CH * 64 + 8;      // of a row that is being merged: 16-byte rows, spread over the banks
-    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256 + (size_t)RG * 2 * 16 * kPitch * 4;
+    static constexpr int kQPitch = CH * 128 + 16;   // bytes of a query row: likewise
+    static constexpr int kQTile = RG * 16 * kQPitch;
+    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 512 + (size_t)RG * 2 * 16 * kPitch * 4 + 2 * kQTile;
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -60,11 +63,43 @@ struct Item {
     bool partial;  // one of several pieces of its rows
 };
 
-__device__ __forceinline__ bool find_item(const Params &p, int work, Item &it) {
+// The first 32 sequences, one per lane, looked up once: with no more than that an item is found without a memory access.
+struct Known {
+    Seq seq;
+    int upto;  // items of this lane's sequence and of those before it
+};
+__device__ __forceinline__ Known look_up(const Params &p) {
+    const int lane = threadIdx.x & 31;
+    Known k = {{0, 0, 0, 0}, 0};
+    if (lane < p.batch) {
+        k.seq = load_seq(p, lane);
+        k.upto = items_of(p, k.seq);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, k.upto, o);
+        if (lane >= o) k.upto += t;
+    }
+    return k;
+}
+
+__device__ __forceinline__ bool find_item(const Params &p, const Known &known, int work, Item &it) {
     int i;
     it.index = work / p.units;
     it.unit = work - it.index * p.units;
-    if (it.index >= p.max_items || !find_seq(p, it.index, [&](const Seq &s) { return items_of(p, s); }, it.seq, i)) return false;
+    if (it.index >= p.max_items) return false;
+    const unsigned hit = __ballot_sync(0xffffffffu, it.index < known.upto);
+    if (hit) {
+        const int src = __ffs(hit) - 1;
+        it.seq.q0 = __shfl_sync(0xffffffffu, known.seq.q0, src);
+        it.seq.nq = __shfl_sync(0xffffffffu, known.seq.nq, src);
+        it.seq.k0 = __shfl_sync(0xffffffffu, known.seq.k0, src);
+        it.seq.nk = __shfl_sync(0xffffffffu, known.seq.nk, src);
+        const int before = __shfl_sync(0xffffffffu, known.upto, max(src - 1, 0));
+        i = it.index - (src > 0 ? before : 0);
+    } else if (p.batch <= 32 || !find_seq(p, it.index, [&](const Seq &s) { return items_of(p, s); }, it.seq, i)) {
+        return false;
+    }
     if (row_tiles(p, it.seq) == 1) {
         it.t0 = 0;
         it.k0 = i * p.part;
@@ -79,18 +114,22 @@ __device__ __forceinline__ bool find_item(const Params &p, int work, Item &it) {
     return true;
 }
 
-// RG groups of 16 rows x 4 groups of 16 keys of each block, a warp each, and a producer warp
+// RG groups of 16 rows x 4 groups of 16 keys of each block, a warp each; a warp that loads keys and values; a warp for items
 template <int CH, int RG>
-__global__ void __launch_bounds__(RG * 128 + 32, 1)
+__global__ void __launch_bounds__(RG * 128 + 64, 1)
 attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p) {
     using Sh = Shape<CH, RG>;
     constexpr int kStages = Sh::kStages, kStage = Sh::kStage, kPitch = Sh::kPitch, kWarps = RG * 4, kD = CH * 64;
     extern __shared__ uint8_t smem_raw[];
+    __shared__ Item s_items[2];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStage);
     uint64_t *empty = full + kStages;
+    uint64_t *item_full = empty + kStages;  // [2] an item's description and query rows are there
+    uint64_t *item_empty = item_full + 2;
+    uint8_t *q_tiles = smem + kStages * kStage + 512;
     // merging: two slots per row group, 16 rows of kD outputs, then the maximum and the sum
-    float *merge = reinterpret_cast<float *>(smem + kStages * kStage + 256);
+    float *merge = reinterpret_cast<float *>(q_tiles + 2 * Sh::kQTile);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -100,13 +139,19 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], kWarps);
         }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&item_full[s], 1);
+            mbar_init(&item_empty[s], kWarps + 1);
+        }
         fence_barrier_init();
         fence_proxy_async();
     }
     __syncthreads();
+    swc_let_next_start();
+    swc_after_previous();
 
     int st = 0;
-    uint32_t ph = 0;
+    uint32_t ph = 0, items = 0;
     const auto next = [&] {
         if (++st == kStages) {
             st = 0;
@@ -115,14 +160,48 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     };
     bool ok = true;
     Item it;
-    if (warp == kWarps) {
+    const auto next_item = [&] {  // false: no more, or a wait ran out
+        ok = warp_wait(&item_full[items & 1], (items >> 1) & 1, p.status, kWaitFull);
+        if (ok) it = s_items[items & 1];
+        return ok && it.unit >= 0;
+    };
+    if (warp == kWarps + 1) {
+        // ------------------------------------------------------------ items
+        const Known known = look_up(p);
+        for (int work = blockIdx.x; ok; work += gridDim.x, items++) {
+            const bool any = find_item(p, known, work, it);
+            if (!any) it.unit = -1;
+            ok = warp_wait(&item_empty[items & 1], ((items >> 1) & 1) ^ 1, p.status, kWaitEmpty);
+            if (!ok) break;
+            if (lane == 0) s_items[items & 1] = it;
+            if (any) {
+                // query rows, 16 bytes at a time; rows of nobody and columns past the width are zeros
+                uint8_t *tile = q_tiles + (items & 1) * Sh::kQTile;
+                constexpr int kPieces = RG * 16 * CH * 8;
+#pragma unroll 8
+                for (int i = lane; i < kPieces; i += 32) {
+                    const int row = i / (CH * 8), c = i % (CH * 8) * 8, tok = row * p.pack_inv >> 16, t = it.t0 + tok;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (tok < p.tokens && t < it.seq.nq && c < p.d)
+                        v = *reinterpret_cast<const uint4 *>(p.q + (size_t)(it.seq.q0 + t) * p.q_row +
+                                                             (size_t)(it.unit * p.pack + row - tok * p.pack) * p.q_head + c);
+                    *reinterpret_cast<uint4 *>(tile + row * Sh::kQPitch + c * 2) = v;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_full[items & 1]);
+            if (!any) break;
+        }
+    } else if (warp == kWarps) {
         // ------------------------------------------------------------ loads
-        for (int work = blockIdx.x; ok && find_item(p, work, it); work += gridDim.x) {
+        for (; ok && next_item(); items++) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[items & 1]);
             const int head_k = it.unit * p.pack / p.group;
             for (int k = it.k0; k < it.k1 && ok; k += kKeys) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, p.status, kWaitEmpty));
+                ok = warp_wait(&empty[st], ph ^ 1, p.status, kWaitEmpty);
                 if (!ok) break;
-                if (lane == 0) {
+                if (elect_one()) {
                     uint8_t *dst = smem + st * kStage;
                     mbar_expect_tx(&full[st], kStage);
                     for (int c = 0; c < CH; c++) tma_load_3d(dst + c * kChunk, &tmK, &full[st], c * 64, head_k, it.seq.k0 + k);
@@ -138,21 +217,20 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         // ldmatrix addresses inside a chunk: keys kg*16 + (0..15); the 16-byte piece is xor-ed with the row by the swizzle
         const int k_row = kg * 16 + (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;   // K: (keys 0-7: d 0-7, 8-15), (keys 8-15: ..)
         const int v_row = kg * 16 + (lane & 15), v_piece = lane >> 4;                            // V: (keys 0-7, 8-15: d 0-7), (.. d 8-15)
-        for (int work = blockIdx.x; ok && find_item(p, work, it); work += gridDim.x) {
+        const int q_row = rg * 16 + (lane & 15), q_piece = lane >> 4;                            // Q: (rows 0-7, 8-15: d 0-7), (.. d 8-15)
+        for (; ok && next_item(); items++) {
             // query fragments, rows g and g + 8 of this row group
             uint32_t qf[kD / 16][4];
+            const uint32_t sq = smem_u32(q_tiles + (items & 1) * Sh::kQTile) + q_row * Sh::kQPitch + q_piece * 16;
+#pragma unroll
+            for (int s = 0; s < kD / 16; s++) ldmatrix4(qf[s], sq + s * 32);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[items & 1]);
             int sees[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int row = rg * 16 + g + h * 8, tok = row / p.pack, t = it.t0 + tok;
-                const bool valid = tok < p.tokens && t < it.seq.nq;
-                sees[h] = valid ? visible(p, it.seq, t) : 0;
-                const __nv_bfloat16 *src = p.q + (size_t)(it.seq.q0 + t) * p.q_row + (size_t)(it.unit * p.pack + row - tok * p.pack) * p.q_head;
-#pragma unroll
-                for (int s = 0; s < kD / 16; s++) {
-                    qf[s][h] = valid && s * 16 + c2 < p.d ? *reinterpret_cast<const uint32_t *>(src + s * 16 + c2) : 0u;
-                    qf[s][h + 2] = valid && s * 16 + c2 + 8 < p.d ? *reinterpret_cast<const uint32_t *>(src + s * 16 + c2 + 8) : 0u;
-                }
+                const int row = rg * 16 + g + h * 8, tok = row * p.pack_inv >> 16, t = it.t0 + tok;
+                sees[h] = tok < p.tokens && t < it.seq.nq ? visible(p, it.seq, t) : 0;
             }
             float o[kD / 8][4];
 #pragma unroll
@@ -160,7 +238,7 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
             for (int k = it.k0; k < it.k1; k += kKeys) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&full[st], ph, p.status, kWaitFull));
+                ok = warp_wait(&full[st], ph, p.status, kWaitFull);
                 if (!ok) break;
                 const uint32_t sk = smem_u32(smem + st * kStage), sv = sk + CH * kChunk;
                 const int first = k + kg * 16;  // this warp's first key
@@ -276,7 +354,7 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             if (kg == 0) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int row = rg * 16 + g + h * 8, tok = row / p.pack, t = it.t0 + tok;
+                    const int row = rg * 16 + g + h * 8, tok = row * p.pack_inv >> 16, t = it.t0 + tok;
                     if (tok >= p.tokens || t >= it.seq.nq) continue;
                     const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
                     const int head = it.unit * p.pack + row - tok * p.pack;
@@ -310,14 +388,20 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     __syncwarp();
 }
 
-// Joins the parts of a row: a CTA per (token, head), warps take parts in turn, then a fixed-order sum over the warps.
+// Joins the parts of a row (token, head): kWarps warps take them in turn, then a fixed-order sum over the warps.  Eight where a row
+// has many parts, one (eight rows per CTA) where it has few.
 // kItems: parts are the items of the token kernel (slot = item), else `parts` of every token of the prompt kernel.
-constexpr int kJoinWarps = 8;
-template <bool kItems>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const Params p, int rows, int parts) {
-    __shared__ float s_o[kJoinWarps][128], s_l[kJoinWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int token = blockIdx.x / p.heads_q, head = blockIdx.x - token * p.heads_q;
+constexpr int kJoinThreads = 256;
+template <bool kItems, int kWarps>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Params p, int rows, int parts) {
+    constexpr int kRowsPerCta = kJoinThreads / 32 / kWarps;
+    __shared__ float s_o[kWarps > 1 ? kWarps : 1][128], s_l[kWarps];
+    const int warp = kWarps > 1 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31;
+    const long long which = (long long)blockIdx.x * kRowsPerCta + (kWarps > 1 ? 0 : threadIdx.x >> 5);
+    swc_let_next_start();
+    swc_after_previous();
+    if (which >= (long long)p.total_q * p.heads_q) return;
+    const int token = (int)(which / p.heads_q), head = (int)(which - (long long)token * p.heads_q);
     size_t slot, step;
     int n;
     if (kItems) {
@@ -360,6 +444,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const P
         slot = (size_t)token * p.heads_q + head;
         step = (size_t)p.total_q * p.heads_q;
     }
+    // this warp's parts are warp, warp + kWarps, ...; several of them are read at once
     float m = -INFINITY;
     for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_lse[slot + i * step]);
 #pragma unroll
@@ -367,33 +452,57 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const P
     const float base = m == -INFINITY ? 0.f : m;
     float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
     const int c = lane * 4;
-#pragma unroll 4
-    for (int i = warp; i < n; i += kJoinWarps) {
-        const size_t at = slot + i * step;
-        const float w = exp2_fast(p.part_lse[at] - base);
-        l += w;
-        if (c < p.d) {
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + at * p.d + c);
-            acc[0] = fmaf(w, v.x, acc[0]);
-            acc[1] = fmaf(w, v.y, acc[1]);
-            acc[2] = fmaf(w, v.z, acc[2]);
-            acc[3] = fmaf(w, v.w, acc[3]);
+    constexpr int kAtOnce = kWarps > 1 ? 16 : 8;
+    for (int first = warp; first < n; first += kWarps * kAtOnce) {
+        const int mine = first + lane * kWarps;  // the first lanes: the weight of a part each
+        const float w_mine = lane < kAtOnce && mine < n ? exp2_fast(p.part_lse[slot + mine * step] - base) : 0.f;
+        float4 v[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const int i = first + k * kWarps;
+            v[k] = i < n && c < p.d ? *reinterpret_cast<const float4 *>(p.part_o + (slot + i * step) * p.d + c) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; k++) {
+            const float w = __shfl_sync(0xffffffffu, w_mine, k);
+            l += w;
+            acc[0] = fmaf(w, v[k].x, acc[0]);
+            acc[1] = fmaf(w, v[k].y, acc[1]);
+            acc[2] = fmaf(w, v[k].z, acc[2]);
+            acc[3] = fmaf(w, v[k].w, acc[3]);
         }
     }
-    *reinterpret_cast<float4 *>(&s_o[warp][c]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    const int d = threadIdx.x;
-    float sum = 0.f;
+    if (kWarps > 1) {
+        *reinterpret_cast<float4 *>(&s_o[warp][c]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (lane == 0) s_l[warp] = l;
+        __syncthreads();
+        if (warp != 0) return;
+        l = 0.f;
+        acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; w++) sum += s_l[w];
-    if (d < p.d) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; w++) v += s_o[w][d];
-        p.o[(size_t)token * p.o_row + (size_t)head * p.o_head + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : v / sum);
+        for (int w = 0; w < kWarps; w++) {
+            const float4 v = *reinterpret_cast<const float4 *>(&s_o[w][c]);
+            l += s_l[w];
+            acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
+        }
     }
-    if (d == 0 && p.lse) p.lse[(size_t)token * p.heads_q + head] = sum == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(sum));
+    if (c < p.d) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint2 w;
+        w.x = pack_bf16(acc[0] * inv, acc[1] * inv);
+        w.y = pack_bf16(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<uint2 *>(p.o + (size_t)token * p.o_row + (size_t)head * p.o_head + c) = w;
+    }
+    if (lane == 0 && p.lse) p.lse[(size_t)token * p.heads_q + head] = l == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
+}
+
+template <bool kItems> int join(swcb200_ctx *ctx, const Params &p, int rows, int parts, bool many) {
+    const long long all = (long long)p.total_q * p.heads_q;
+    if (many)
+        SWC_CUDA(ctx, swc_launch_early(attention_join_kernel<kItems, 8>, (unsigned)all, kJoinThreads, 0, ctx->stream, 1, p, rows, parts));
+    else
+        SWC_CUDA(ctx, swc_launch_early(attention_join_kernel<kItems, 1>, (unsigned)((all + 7) / 8), kJoinThreads, 0, ctx->stream, 1, p, rows, parts));
+    return swc_check_launch(ctx, "attention_bf16");
 }
 
 template <int CH, int RG>
@@ -402,7 +511,7 @@ int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmK, const CUte
     SWC_CUDA(ctx, cudaFuncSetAttribute(attention_token_kernel<CH, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const long long work = (long long)max_items * p.units;
     const unsigned grid = (unsigned)(work < ctx->sm_count ? work : ctx->sm_count);
-    attention_token_kernel<CH, RG><<<grid, RG * 128 + 32, smem, ctx->stream>>>(tmK, tmV, p);
+    SWC_CUDA(ctx, swc_launch_early(attention_token_kernel<CH, RG>, grid, RG * 128 + 64, smem, ctx->stream, 1, tmK, tmV, p));
     return swc_check_launch(ctx, "attention_bf16");
 }
 
@@ -415,11 +524,7 @@ int swc_attention_token(swcb200_ctx *ctx, Params &p, const CUtensorMap &tmK, con
     else
         rc = rows == 16 ? launch<1, 1>(ctx, p, tmK, tmV, max_items) : rows == 32 ? launch<1, 2>(ctx, p, tmK, tmV, max_items) : launch<1, 4>(ctx, p, tmK, tmV, max_items);
     if (rc || p.part >= p.total_k) return rc;  // no sequence has more than one part
-    attention_join_kernel<true><<<(unsigned)p.total_q * p.heads_q, kJoinWarps * 32, 0, ctx->stream>>>(p, rows, 0);
-    return swc_check_launch(ctx, "attention_bf16");
+    return join<true>(ctx, p, rows, 0, p.total_k / p.batch > 16ll * p.part);
 }
 
-int swc_attention_join_parts(swcb200_ctx *ctx, Params &p, int parts) {
-    attention_join_kernel<false><<<(unsigned)p.total_q * p.heads_q, kJoinWarps * 32, 0, ctx->stream>>>(p, 0, parts);
-    return swc_check_launch(ctx, "attention_bf16");
-}
+int swc_attention_join_parts(swcb200_ctx *ctx, Params &p, int parts) { return join<false>(ctx, p, 0, parts, false); }

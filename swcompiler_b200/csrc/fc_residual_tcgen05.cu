@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     uint64_t *done = empty + p.stages;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(done + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // warp: known to be uniform
     const uint32_t tmem_cols = p.bn < 32 ? 32u : (uint32_t)p.bn;
     const uint32_t rank = p.splits > 1 ? cluster_ctarank() : 0;
     const int tile = blockIdx.x / p.splits;
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     swc_let_next_start();
     swc_after_previous();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_holder;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     bool failed = false;
     // epilogue warps: a row of the tile (an output column) per thread, in the lane quarter that the warp may read
     const int row = (warp & 3) * 32 + lane, col = tn * BM + row;
@@ -206,31 +206,32 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = idesc_bf16_f32(BM, p.bn);
-            int st = 0;
-            uint32_t ph = 0;
-            for (int kb = kb0; kb < kb1; kb++) {
-                if (!mbar_wait(&full[st], ph, p.status, kWaitFull)) {
-                    failed = true;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t sw = smem_u32(smem + (size_t)st * stage_bytes);
+        const uint32_t idesc = idesc_bf16_f32(BM, p.bn);
+        const uint32_t dw0 = desc_low(smem_u32(smem), 16), da0 = desc_low(smem_u32(smem + W_BYTES), 16);
+        int st = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (!warp_wait(&full[st], ph, p.status, kWaitFull)) {
+                failed = true;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t off = (uint32_t)st * (stage_bytes >> 4);
+            if (elect_one()) {
 #pragma unroll
-                for (int b = 0; b < kSub; b++) {
-                    const uint64_t dw = smem_desc_sw128(sw + b * block_bytes), da = smem_desc_sw128(sw + b * block_bytes + W_BYTES);
+                for (int b = 0; b < kSub; b++)
 #pragma unroll
                     for (int j = 0; j < BK / UMMA_K; j++)
-                        umma_bf16(tmem_base, dw + 2 * j, da + 2 * j, idesc, (uint32_t)(kb != kb0 || b + j != 0));
-                }
+                        umma_bf16_words(tmem_base, dw0 + off + b * (block_bytes >> 4) + 2 * j, da0 + off + b * (block_bytes >> 4) + 2 * j, idesc,
+                                        kb != kb0 || b + j != 0);
                 umma_commit(&empty[st]);
-                if (++st == p.stages) {
-                    st = 0;
-                    ph ^= 1;
-                }
+                if (kb + 1 == kb1) umma_commit(done);
             }
-            if (!failed) umma_commit(done);
+            __syncwarp();
+            if (++st == p.stages) {
+                st = 0;
+                ph ^= 1;
+            }
         }
     } else {
         bool ok = true;
@@ -286,8 +287,10 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
                 finish_joined<2>(p, mine, slot, token0, col, bias);
             else if (own < 16)
                 for (int t = 0; t < own; t += 4) finish_joined<4>(p, mine + t * BM, slot, token0 + t, col, bias);
+            else if (own < 32)
+                finish_joined<16>(p, mine, slot, token0, col, bias);
             else
-                for (int t = 0; t < own; t += 16) finish_joined<16>(p, mine + t * BM, slot, token0 + t, col, bias);
+                for (int t = 0; t < own; t += 32) finish_joined<32>(p, mine + t * BM, slot, token0 + t, col, bias);
         }
     }
     if (warp == 1) {
@@ -418,7 +421,7 @@ fc_res_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     uint64_t *tmem_empty = tmem_full + 2;
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(tmem_empty + 2);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;  // warp: known to be uniform
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int num_tiles = p.tiles_m * p.tiles_n;
@@ -450,7 +453,7 @@ fc_res_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     swc_let_next_start();
     swc_after_previous();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_holder;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     bool failed = false;
 
     if (warp == 0) {
@@ -480,38 +483,38 @@ fc_res_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             }
         }
     } else if (warp == 1) {
-        if (leader && lane == 0) {
+        if (leader) {
             const uint32_t idesc = idesc_bf16_f32(2 * BM, p.bn);
-            const uint64_t dw0 = smem_desc_sw128(smem_u32(smem)), da0 = smem_desc_sw128(smem_u32(smem + W_BYTES));
+            const uint32_t dw0 = desc_low(smem_u32(smem), 16), da0 = desc_low(smem_u32(smem + W_BYTES), 16);
             int st = 0;
             uint32_t ph = 0, it = 0;
             for (int t = cluster_id; t < num_tiles && !failed; t += num_clusters, it++) {
                 const uint32_t buf = it & 1, aph = (it >> 1) & 1;
-                if (!mbar_wait(&tmem_empty[buf], aph ^ 1, p.status, kWaitTmemEmpty)) {
+                if (!warp_wait(&tmem_empty[buf], aph ^ 1, p.status, kWaitTmemEmpty)) {
                     failed = true;
                     break;
                 }
-                tc_fence_after();
                 const uint32_t d_tmem = tmem_base + buf * BN_MAX;
                 for (int kb = 0; kb < kblocks; kb++) {
-                    if (!mbar_wait(&full[st], ph, p.status, kWaitFull)) {
+                    if (!warp_wait(&full[st], ph, p.status, kWaitFull)) {
                         failed = true;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t off = (uint64_t)st * (kPairStageBytes >> 4);
-                    const uint64_t dw = dw0 + off, da = da0 + off;
-                    umma_bf16_pair(d_tmem, dw, da, idesc, (uint32_t)(kb != 0));
-                    umma_bf16_pair(d_tmem, dw + 2, da + 2, idesc, 1u);
-                    umma_bf16_pair(d_tmem, dw + 4, da + 4, idesc, 1u);
-                    umma_bf16_pair(d_tmem, dw + 6, da + 6, idesc, 1u);
-                    umma_commit_pair(&empty[st], 3);
+                    const uint32_t off = (uint32_t)st * (kPairStageBytes >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < BK / UMMA_K; j++)
+                            umma_bf16_pair_words(d_tmem, dw0 + off + 2 * j, da0 + off + 2 * j, idesc, kb != 0 || j != 0);
+                        umma_commit_pair(&empty[st], 3);
+                        if (kb + 1 == kblocks) umma_commit_pair(&tmem_full[buf], 3);
+                    }
+                    __syncwarp();
                     if (++st == kPairStages) {
                         st = 0;
                         ph ^= 1;
                     }
                 }
-                if (!failed) umma_commit_pair(&tmem_full[buf], 3);
             }
         }
     } else {

@@ -227,6 +227,35 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint
         : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The same with the descriptors as words, of which only the low ones differ (kDescHigh: 8 rows 1024 bytes apart, version 1, 128-byte
+// swizzle).  For issuing loops that a whole warp runs and one thread, chosen by elect_one(), executes: there the compiler keeps
+// operands that are the same in all lanes in uniform registers, as the instruction wants them.  Behind `lane == 0`, or with 64-bit
+// descriptors that it computes per instruction, an instruction took 110 to 160 cycles to issue instead of 64.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+// low word: address, and the leading offset in bytes, which K-major operands do not use
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t leading) { return ((saddr & 0x3FFFF) >> 4) | (leading >> 4 << 16); }
+__device__ __forceinline__ void umma_bf16_words(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(kDescHigh), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_bf16_pair_words(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(kDescHigh), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+// a whole warp waits, and gives up together
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int *status, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+}
 // mbarrier arrives once every tcgen05.mma issued so far by this thread has completed
 __device__ __forceinline__ void umma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
