@@ -34,11 +34,12 @@ int make_plan(swcb200_ctx *ctx, const swcb200_attention *a, Plan &pl) {
         while (pl.rows < pl.pack * average) pl.rows *= 2;
         pl.tokens = pl.rows / pl.pack;
         pl.units = a->heads_q / pl.pack;
-        // keys per item: one item per SM as long as that is no more than 512 keys (256 KiB of cache at width 128, about 6 us of an
-        // SM's share of HBM); larger ones only where items would number more than 32 per SM
+        // Keys per item.  One item for each of two CTAs per SM while that is no more than 2048 keys: one wave, and the fewest parts
+        // to join (one sequence of 65536 keys: 59 -> 52 us).  Else 512, which evens out lengths that differ (256 KiB of cache at
+        // width 128, about 6 us of an SM's share of HBM), and more only where items would number beyond 32 per SM.
         const long long keys = (long long)a->total_k * pl.units;
-        long long part = keys / ctx->sm_count;
-        part = part < 512 ? part : 512;
+        long long part = keys / (2ll * ctx->sm_count);
+        if (part > 2048) part = 512;
         part = part > keys / (32ll * ctx->sm_count) ? part : keys / (32ll * ctx->sm_count);
         pl.part = (int)((part + 63) / 64 * 64);
         if (pl.part < 64) pl.part = 64;

@@ -22,7 +22,8 @@ constexpr int kChunk = kKeys * 128;   // bytes of a 64-wide chunk of a block
 
 template <int CH, int RG> struct Shape {
     static constexpr int kStage = 2 * CH * kChunk;  // K and V of a block
-    static constexpr int kStages = CH == 1 ? 8 : RG < 4 ? 5 : 3;
+    static constexpr int kCtas = RG == 1 ? 2 : 1;   // per SM
+    static constexpr int kStages = RG == 1 ? (CH == 1 ? 4 : 2) : CH == 1 ? 8 : RG < 4 ? 5 : 3;
     static constexpr int kPitch = CH * 64 + 8;      // of a row that is being merged: 16-byte rows, spread over the banks
     static constexpr int kQPitch = CH * 128 + 16;   // bytes of a query row: likewise
     static constexpr int kQTile = RG * 16 * kQPitch;
@@ -116,7 +117,7 @@ __device__ __forceinline__ bool find_item(const Params &p, const Known &known, i
 
 // RG groups of 16 rows x 4 groups of 16 keys of each block, a warp each; a warp that loads keys and values; a warp for items
 template <int CH, int RG>
-__global__ void __launch_bounds__(RG * 128 + 64, 1)
+__global__ void __launch_bounds__(RG * 128 + 64, Shape<CH, RG>::kCtas)
 attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Params p) {
     using Sh = Shape<CH, RG>;
     constexpr int kStages = Sh::kStages, kStage = Sh::kStage, kPitch = Sh::kPitch, kWarps = RG * 4, kD = CH * 64;
@@ -510,7 +511,8 @@ int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmK, const CUte
     const size_t smem = Shape<CH, RG>::kSmem;
     SWC_CUDA(ctx, cudaFuncSetAttribute(attention_token_kernel<CH, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const long long work = (long long)max_items * p.units;
-    const unsigned grid = (unsigned)(work < ctx->sm_count ? work : ctx->sm_count);
+    const long long slots = (long long)ctx->sm_count * Shape<CH, RG>::kCtas;
+    const unsigned grid = (unsigned)(work < slots ? work : slots);
     SWC_CUDA(ctx, swc_launch_early(attention_token_kernel<CH, RG>, grid, RG * 128 + 64, smem, ctx->stream, 1, tmK, tmV, p));
     return swc_check_launch(ctx, "attention_bf16");
 }

@@ -467,6 +467,8 @@ class Backend:
         if tv != tk or hv != hkv or dv != d or dk != d or not fits:
             raise ValueError("attention_bf16: q, out [total_q, heads_q, d] and k, v [total_k, heads_kv, d]")
         batch = q_offsets.numel() - 1
+        if batch < 0:
+            raise ValueError("attention_bf16: offsets have batch + 1 elements")
         p_qo, p_ko = self._lengths(what, q_offsets, batch + 1), self._lengths(what, k_offsets, batch + 1)
         p_kl = 0 if k_lens is None else self._lengths(what, k_lens, batch)
         p_lse = 0
