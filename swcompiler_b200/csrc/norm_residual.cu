@@ -280,10 +280,10 @@ SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, co
     SWC_REQUIRE(ctx, known_dtype(d->x_dtype) && (!d->residual || known_dtype(d->residual_dtype)) &&
                 (!d->gate || known_dtype(d->gate_dtype)) && (!d->sum || known_dtype(d->sum_dtype)) &&
                 (!d->y || known_dtype(d->y_dtype)), SWCB200_ERR_BAD_ARG, "norm_residual: tensors are fp32 or bf16");
-    SWC_REQUIRE(ctx, (d->y != nullptr) == (d->pre.kind != SWCB200_NORM_NONE), SWCB200_ERR_BAD_ARG,
-                "norm_residual: y and the norm that writes it go together");
     SWC_REQUIRE(ctx, d->gate_rows >= 0, SWCB200_ERR_BAD_ARG, "norm_residual: negative gate_rows");
     if (rows == 0) return SWCB200_OK;
+    SWC_REQUIRE(ctx, (d->y != nullptr) == (d->pre.kind != SWCB200_NORM_NONE), SWCB200_ERR_BAD_ARG,
+                "norm_residual: y and the norm that writes it go together");
     SWC_REQUIRE(ctx, d->x && (d->sum || d->y), SWCB200_ERR_BAD_ARG, "norm_residual: null tensor");
     const size_t c = (size_t)cols;
     SWC_REQUIRE(ctx, rows == 1 || (d->ldx >= c && (!d->residual || d->ld_residual >= c) && (!d->sum || d->ld_sum >= c) &&
