@@ -41,34 +41,55 @@ struct RowParams {
     NormParams post, pre;
 };
 
-// How a chunk is read: not at all, as bf16, as fp32.  The reads are predicated inside one statement, so that a thread's chunks
-// are all requested before the first is converted (a branch on the type would wait for each chunk in turn).
+// How a tensor is read: not at all, as bf16, as fp32.
 enum : int { kSkip = 0, kBf16 = 1, kF32 = 2 };
 
-template <int kVec> __device__ __forceinline__ void load_chunk(const void *p, size_t i, int how, uint32_t (&r)[kVec]) {
-    const void *at = reinterpret_cast<const char *>(p) + i * (how == kF32 ? 4 : 2);
-    if constexpr (kVec == 8) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) r[j] = 0u;
+template <int kVec, int kType> __device__ __forceinline__ void load_chunk(const void *p, size_t i, bool in, uint32_t (&r)[kVec]) {
+    if constexpr (kVec == 8 && kType == kBf16)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3])
+                     : "l"(reinterpret_cast<const __nv_bfloat16 *>(p) + i), "r"((uint32_t)in));
+    else if constexpr (kVec == 8)
         asm volatile(
-            "{\n\t.reg .pred h, f;\n\t"
-            "setp.eq.s32 h, %9, 1;\n\tsetp.eq.s32 f, %9, 2;\n\t"
-            "@h ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%8];\n\t"
-            "@f ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t}"
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %9, 0;\n\t"
+            "@p ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t}"
             : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-            : "l"(at), "r"(how));
-    } else {
-        r[0] = 0u;
-        asm volatile(
-            "{\n\t.reg .pred h, f;\n\t"
-            "setp.eq.s32 h, %2, 1;\n\tsetp.eq.s32 f, %2, 2;\n\t"
-            "@h ld.global.u16 %0, [%1];\n\t"
-            "@f ld.global.b32 %0, [%1];\n\t}"
-            : "+r"(r[0])
-            : "l"(at), "r"(how));
+            : "l"(reinterpret_cast<const float *>(p) + i), "r"((uint32_t)in));
+    else if constexpr (kType == kBf16)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}"
+                     : "+r"(r[0])
+                     : "l"(reinterpret_cast<const __nv_bfloat16 *>(p) + i), "r"((uint32_t)in));
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
+                     : "+r"(r[0])
+                     : "l"(reinterpret_cast<const float *>(p) + i), "r"((uint32_t)in));
+}
+// All chunks of a thread, as they are: requested one behind the other, and none converted before the last is requested.  kType: the
+// type where the kernel is compiled for it (selecting it per element took a third of the instructions), 0 for either.  (One
+// statement with two predicated loads into a register, one of them never executed, waits for the first all the same: 20000 rows
+// of 1003 took 150 us that way.)
+template <int kVec, int kN, int kType>
+__device__ __forceinline__ void load_chunks(const void *p, size_t at, int how, int tpr, int cols, int tid, uint32_t (&r)[kN][kVec]) {
+#pragma unroll
+    for (int i = 0; i < kN; i++)
+#pragma unroll
+        for (int e = 0; e < kVec; e++) r[i][e] = 0u;
+    if (kType != kF32 && how == kBf16) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int c = (i * tpr + tid) * kVec;
+            load_chunk<kVec, kBf16>(p, at + c, c < cols, r[i]);
+        }
+    } else if (kType != kBf16 && how == kF32) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int c = (i * tpr + tid) * kVec;
+            load_chunk<kVec, kF32>(p, at + c, c < cols, r[i]);
+        }
     }
 }
-template <int kVec> __device__ __forceinline__ float element(const uint32_t (&r)[kVec], int e, bool is16) {
+template <int kVec, int kType> __device__ __forceinline__ float element(const uint32_t (&r)[kVec], int e, int how) {
+    const bool is16 = (kType ? kType : how) == kBf16;
     if (kVec == 1) return __uint_as_float(is16 ? r[0] << 16 : r[0]);
     const uint32_t h = e & 1 ? r[e / 2] & 0xffff0000u : r[e / 2] << 16;
     return __uint_as_float(is16 ? h : r[e]);
@@ -128,9 +149,13 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float *red) {
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = lane < warps ? red[lane] : 0.f;
+    v = 0.f;  // (the other sums of a few warps: reads of one address are cheaper than another round of shuffles)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    for (int i = 0; i < kMaxThreads / 32; i += 4)
+        if (i < warps) {
+            const float4 q = *reinterpret_cast<const float4 *>(red + i);
+            v += (q.x + (i + 1 < warps ? q.y : 0.f)) + ((i + 2 < warps ? q.z : 0.f) + (i + 3 < warps ? q.w : 0.f));
+        }
     return v;
 }
 
@@ -170,11 +195,13 @@ __device__ __forceinline__ void store1(void *p, size_t i, bool is16, float v) {
         reinterpret_cast<float *>(p)[i] = v;
 }
 
-template <int kVec, int kN, bool kCta>
-__global__ void __launch_bounds__(kCta ? kMaxThreads : 128) norm_residual_kernel(const RowParams p) {
+template <int kVec, int kN, bool kCta, int kX, int kR>
+// (up to 16 elements a thread come with 256 threads at most, and four such CTAs keep an SM busier than three)
+__global__ void __launch_bounds__(!kCta ? 128 : kN * kVec <= 16 ? 256 : kMaxThreads, kCta && kN * kVec <= 16 ? 4 : 1)
+norm_residual_kernel(const RowParams p) {
     swc_let_next_start();
     swc_after_previous();
-    __shared__ float red[128];  // one part for each of the four row sums: no barrier between reading one and writing the next
+    __shared__ alignas(16) float red[128];  // one part for each of the four row sums: no barrier between reading one and writing the next
     const int tid = kCta ? threadIdx.x : threadIdx.x & (p.tpr - 1);
     const int rows_per_cta = kCta ? 1 : blockDim.x / p.tpr;
     const long long row = (long long)blockIdx.x * rows_per_cta + (kCta ? 0 : threadIdx.x / p.tpr);
@@ -182,34 +209,22 @@ __global__ void __launch_bounds__(kCta ? kMaxThreads : 128) norm_residual_kernel
     const int cols = row < p.rows ? p.cols : 0;
     float t[kN * kVec];
     uint32_t x[kN][kVec], r[kN][kVec];
+    load_chunks<kVec, kN, kX>(p.x, (size_t)row * p.ldx, p.x_how, p.tpr, cols, tid, x);
+    load_chunks<kVec, kN, kR>(p.residual, (size_t)row * p.ldr, p.r_how, p.tpr, cols, tid, r);
 #pragma unroll
-    for (int i = 0; i < kN; i++) {
-        const int c = (i * p.tpr + tid) * kVec;
-        load_chunk<kVec>(p.x, (size_t)row * p.ldx + c, c < cols ? p.x_how : kSkip, x[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kN; i++) {
-        const int c = (i * p.tpr + tid) * kVec;
-        load_chunk<kVec>(p.residual, (size_t)row * p.ldr + c, c < cols ? p.r_how : kSkip, r[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < kN * kVec; j++) t[j] = element<kVec>(x[j / kVec], j % kVec, p.x_how == kBf16);
+    for (int j = 0; j < kN * kVec; j++) t[j] = element<kVec, kX>(x[j / kVec], j % kVec, p.x_how);
     if (p.post.kind) norm_row<kVec, kN, kCta>(p.post, p, t, tid, red);
 #pragma unroll
     for (int j = 0; j < kN * kVec; j++) t[j] *= p.scale;
     if (p.gate) {
         const size_t base = p.gate_rows ? (size_t)(row / p.gate_rows) * p.ldg : 0;
+        load_chunks<kVec, kN, 0>(p.gate, base, p.g_how, p.tpr, cols, tid, x);
 #pragma unroll
-        for (int i = 0; i < kN; i++) {
-            const int c = (i * p.tpr + tid) * kVec;
-            load_chunk<kVec>(p.gate, base + c, c < cols ? p.g_how : kSkip, x[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < kN * kVec; j++) t[j] *= element<kVec>(x[j / kVec], j % kVec, p.g_how == kBf16);
+        for (int j = 0; j < kN * kVec; j++) t[j] *= element<kVec, 0>(x[j / kVec], j % kVec, p.g_how);
     }
     if (p.residual) {
 #pragma unroll
-        for (int j = 0; j < kN * kVec; j++) t[j] += element<kVec>(r[j / kVec], j % kVec, p.r_how == kBf16);
+        for (int j = 0; j < kN * kVec; j++) t[j] += element<kVec, kR>(r[j / kVec], j % kVec, p.r_how);
     }
     if (p.sum) {
 #pragma unroll
@@ -244,12 +259,18 @@ __global__ void __launch_bounds__(kCta ? kMaxThreads : 128) norm_residual_kernel
     }
 }
 
-template <int kVec, bool kCta> cudaError_t launch(int n, unsigned grid, int threads, cudaStream_t s, const RowParams &p) {
+template <int kVec, bool kCta, int kX, int kR> cudaError_t launch_types(int n, unsigned grid, int threads, cudaStream_t s, const RowParams &p) {
     constexpr int k = kVec == 8 ? 1 : 8;  // chunks of one element come in eights
-    const auto kernel = n <= k       ? norm_residual_kernel<kVec, k, kCta>
-                        : n <= 2 * k ? norm_residual_kernel<kVec, 2 * k, kCta>
-                                     : norm_residual_kernel<kVec, 4 * k, kCta>;
+    const auto kernel = n <= k       ? norm_residual_kernel<kVec, k, kCta, kX, kR>
+                        : n <= 2 * k ? norm_residual_kernel<kVec, 2 * k, kCta, kX, kR>
+                                     : norm_residual_kernel<kVec, 4 * k, kCta, kX, kR>;
     return swc_launch_early(kernel, grid, (unsigned)threads, 0, s, 1, p);
+}
+template <bool kCta> cudaError_t launch(bool vec, int n, unsigned grid, int threads, cudaStream_t s, const RowParams &p) {
+    if (!vec) return launch_types<1, kCta, 0, 0>(n, grid, threads, s, p);
+    if (p.x_how == kBf16)
+        return p.r_how == kF32 ? launch_types<8, kCta, kBf16, kF32>(n, grid, threads, s, p) : launch_types<8, kCta, kBf16, kBf16>(n, grid, threads, s, p);
+    return p.r_how == kF32 ? launch_types<8, kCta, kF32, kF32>(n, grid, threads, s, p) : launch_types<8, kCta, kF32, kBf16>(n, grid, threads, s, p);
 }
 
 bool known_dtype(int d) { return d == SWCB200_F32 || d == SWCB200_BF16; }
@@ -345,7 +366,7 @@ SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, co
         const int per_cta = 128 / p.tpr;
         const unsigned grid = (unsigned)((rows + per_cta - 1) / per_cta);
         const int n = (chunks + p.tpr - 1) / p.tpr;
-        SWC_CUDA(ctx, (vec ? launch<8, false>(n, grid, 128, ctx->stream, p) : launch<1, false>(n, grid, 128, ctx->stream, p)));
+        SWC_CUDA(ctx, launch<false>(vec, n, grid, 128, ctx->stream, p));
     } else {
         // 256 threads where a thread can hold its share: 8192 rows of 4096 in 68 us against 78 with 128 and 83 with 512 threads
         int per = (chunks + 255) / 256;
@@ -354,8 +375,7 @@ SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, co
         threads = (threads + 31) / 32 * 32;
         p.tpr = threads;
         const int n = (chunks + threads - 1) / threads;
-        SWC_CUDA(ctx, (vec ? launch<8, true>(n, (unsigned)rows, threads, ctx->stream, p)
-                           : launch<1, true>(n, (unsigned)rows, threads, ctx->stream, p)));
+        SWC_CUDA(ctx, launch<true>(vec, n, (unsigned)rows, threads, ctx->stream, p));
     }
     return swc_check_launch(ctx, "norm_residual");
 }
