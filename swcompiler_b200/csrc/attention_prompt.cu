@@ -16,8 +16,14 @@
 //     launch control), finds their sequence and hands the item to the other warps ahead of time.
 // Tensor memory: scores 2 x 128 columns, outputs 2 x 128 columns, all 512.  Head widths up to 64 use one 128-byte chunk per row,
 // up to 128 two; TMA fills the rest with zeros.
-// What bounds it: at width 128 a block of a tile costs 1024 cycles of tensor pipe and as many of the exponential unit (16 per
-// cycle); at width 64 the exponentials alone take twice the pipe's time.
+// What bounds it: a block of a tile costs 1024 cycles of tensor pipe at width 128 (512 at 64) and 1024 of the exponential unit (16
+// per cycle), but the two tiles together take some 3200 cycles per block: a tile's softmax (1900) and the products between two
+// of them (1030) are a chain, as there is room for one block of scores per tile.  At width 128 and long prompts that is also
+// where the power limit sets the clock: 16 heads, 4 key heads, 16384 keys, causal: 855 us, 1290 TFLOP/s, 0.80 of the burst and
+// 0.96 of the sustained bf16 rate measured here; width 64: 800 us.  Prompts of a few hundred tokens spend as long at the items'
+// ends (first scores, last output) as in between: 64 sequences of 197, 16 heads of 64: 57 us, a quarter of the bytes' rate.
+// Measured and not kept: scores of blocks of 64 keys two ahead (the instructions around twice as many blocks cost what the chain
+// does), an issuing warp per tile (the tiles fall into step: 1088 us).
 #include "attention_common.cuh"
 
 namespace {
@@ -90,7 +96,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // The weights of 32 keys of a row: powers of two of s * scale - base, as bf16 pairs into tensor memory; their sum is added to l.
 // (The exponential unit gives 16 values per cycle and SM; a part of them on the FMA pipe, by a polynomial of degree 3, was measured
-// and is slower at every share: 905 us without against 941 with a quarter, 16384 keys of width 128.)
+// and is slower at every share: 905 us without against 941 with a quarter of them, 16384 keys of width 128.)
 __device__ __forceinline__ void weights(const float *s, uint64_t scale, uint64_t minus_base, uint32_t t_p, uint64_t &l) {
     uint32_t w[16];
 #pragma unroll
@@ -112,14 +118,6 @@ template <int kCount> __device__ __forceinline__ float largest(const float *s) {
         for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], s[c + i], s[c + 4 + i]);
     const float a = max3(mx[0], s[kCount - 4], s[kCount - 3]), b = max3(mx[1], s[kCount - 2], s[kCount - 1]);
     return max3(max3(a, b, mx[2]), mx[3], mx[3]);
-}
-
-// 32 scores of a row, those from `seen` on out of sight
-__device__ __forceinline__ void load_masked(uint32_t t_s, int seen, float (&s)[32]) {
-    tmem_ld_32x32(t_s, reinterpret_cast<uint32_t(&)[32]>(s));
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 32; i++) s[i] = i < seen ? s[i] : -INFINITY;
 }
 
 // Takes over a block of the grid that has not started: 16 bytes of answer land at `result`, counted on `bar`.
@@ -602,9 +600,6 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     break;
                 }
                 tc_fence_after();
-                // A block that every row sees is held in registers.  Of one that is seen in part the chunks of 32 keys that some row
-                // sees are taken in turn, twice, from tensor memory: a compact loop (masks for all 128 keys, unrolled, made the
-                // softmax warps wait for instructions).
                 const int keys = one_sees - j * kKeys, mine = sees - j * kKeys;
                 const bool whole = all_see - j * kKeys >= kKeys;
                 float s[kKeys];
@@ -639,46 +634,34 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     const float b = m == -INFINITY ? 0.f : -m * p.scale_log2;
                     return pair(b, b);
                 };
-                if (whole) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) tmem_ld_32x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
-                    tmem_ld_wait();
-                    if (j == 0) grow(largest<kKeys>(s));
-                    // The first half's weights are taken relative to the maximum so far, while this block's is looked for: that is off
-                    // the path between the products, and rarely are they to be done again.
-                    uint64_t l_half;
+                for (int c = 0; c < 4; c++) tmem_ld_32x32(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+                tmem_ld_wait();
+                if (!whole) {
+#pragma unroll
+                    for (int c = 0; c < kKeys; c++) s[c] = c < mine ? s[c] : -INFINITY;
+                }
+                if (j == 0) grow(largest<kKeys>(s));
+                // The first half's weights are taken relative to the maximum so far, while this block's is looked for: that is off the
+                // path between the products, and rarely are they to be done again.
+                uint64_t l_half;
 #pragma unroll 1
-                    for (int pass = 0;; pass++) {
-                        l_half = l;
-                        const uint64_t b = base();
-                        weights(s, scale2, b, t_s, l_half);
-                        const float top = largest<kKeys>(s);
-                        weights(s + 32, scale2, b, t_s + 16, l_half);
-                        const bool stays = (top - m) * p.scale_log2 <= kSlack || top == -INFINITY;
-                        if (pass == 1 || __all_sync(0xffffffffu, stays)) break;
-                        grow(top);
-                    }
-                    l = l_half;
-                    publish(&p_half[h]);
+                for (int pass = 0;; pass++) {
+                    l_half = l;
+                    const uint64_t b = base();
+                    weights(s, scale2, b, t_s, l_half);
+                    const float top = largest<kKeys>(s);
+                    weights(s + 32, scale2, b, t_s + 16, l_half);
+                    const bool stays = (top - m) * p.scale_log2 <= kSlack || top == -INFINITY;
+                    if (pass == 1 || __all_sync(0xffffffffu, stays)) break;
+                    grow(top);
+                }
+                l = l_half;
+                publish(&p_half[h]);
+                if (keys > 64) {  // (weights of keys that no row of the tile sees are not multiplied either)
                     const uint64_t b = base();
                     weights(s + 64, scale2, b, t_s + 32, l);
                     weights(s + 96, scale2, b, t_s + 48, l);
-                } else {
-                    float top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < kKeys && c < keys; c += 32) {
-                        load_masked(t_s + c, mine - c, reinterpret_cast<float(&)[32]>(s[0]));
-                        top = max3(top, top, largest<32>(s));
-                    }
-                    grow(top);
-                    const uint64_t b = base();
-                    // (weights of a chunk overwrite scores of chunks that have been read: two columns of scores become one)
-#pragma unroll 1
-                    for (int c = 0; c < kKeys && c < keys; c += 32) {
-                        load_masked(t_s + c, mine - c, reinterpret_cast<float(&)[32]>(s[0]));
-                        weights(s, scale2, b, t_s + c / 2, l);
-                    }
-                    publish(&p_half[h]);
                 }
                 publish(&p_full[h]);
             }
