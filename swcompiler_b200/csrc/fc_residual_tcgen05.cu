@@ -129,7 +129,7 @@ __device__ __forceinline__ void finish_joined(const FcrParams &p, const float *m
     finish<kTok>(p, v, token, col, bias);
 }
 
-constexpr int kSplitThreads = 192;  // TMA warp, MMA warp, 4 epilogue warps
+constexpr int kSplitThreads = 320;  // TMA warp, MMA warp, 8 epilogue warps: two per lane quarter of tensor memory
 
 // shared memory: `stages` x (weight tile, token tile), then barriers; once every CTA of the cluster has multiplied its last stage
 // the ring becomes the join's slots, [splits][own][128 rows] fp32 with own = BN / splits tokens: a warp's store to another CTA is
@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     bool failed = false;
     // epilogue warps: a row of the tile (an output column) per thread, in the lane quarter that the warp may read
-    const int row = (warp & 3) * 32 + lane, col = tn * BM + row;
+    const int row = (warp & 3) * 32 + lane, col = tn * BM + row, half = (warp - 2) >> 2;
+    const int own = p.bn / p.splits;  // tokens that this CTA joins: a power of two, at least 2
     const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
 
     if (warp == 0) {
@@ -234,13 +235,23 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
             }
         }
     } else {
+        // the residual's rows are brought as near as L2 while the products run
+        if (p.residual && col - lane < p.n) {
+            const int first = p.splits > 1 ? (int)rank * own : 0, count = min(p.splits > 1 ? own : p.bn, p.m - tm * p.bn - first);
+            const size_t e = p.r16 ? 2 : 4;
+            for (int t = half * 32 + lane; t < count; t += 64) {
+                const char *at = reinterpret_cast<const char *>(p.residual) + ((size_t)(tm * p.bn + first + t) * p.ldr + col - lane) * e;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (min(31, p.n - 1 - (col - lane))) * e));
+            }
+        }
         bool ok = true;
         if (lane == 0) ok = mbar_wait(done, 0, p.status, kWaitTmemFull);
         failed = !__shfl_sync(0xffffffffu, ok, 0);
         tc_fence_after();
         if (!failed && p.splits == 1) {
             const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
-            for (int c0 = 0; c0 < p.bn; c0 += 16) {
+            for (int c0 = half * 16; c0 < p.bn; c0 += 32) {
                 if (tm * p.bn + c0 >= p.m) break;
                 uint32_t r[16];
                 float acc[16];
@@ -259,12 +270,12 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
     __syncthreads();
     if (p.splits > 1) {
         cluster_sync();  // every CTA has read its last stage: the rings may be overwritten
-        const int own = p.bn / p.splits, own_log2 = 31 - __clz(own);  // a power of two, at least 2
+        const int own_log2 = 31 - __clz(own);
         if (warp >= 2) {
             // this CTA's partial sums go to the CTAs that own the tokens, slot `rank`
             tc_fence_after();
             const uint32_t mine = smem_u32(slots + (int)rank * own * BM + row);
-            for (int c0 = 0; c0 < p.bn; c0 += 16) {
+            for (int c0 = half * 16; c0 < p.bn; c0 += 32) {
                 if (tm * p.bn + c0 >= p.m) break;
                 uint32_t r[16];
                 tmem_ld_32x16(taddr + c0, r);
@@ -281,16 +292,18 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
         cluster_sync();  // all partial sums have arrived
         if (warp >= 2) {
             const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
-            const float *mine = slots + row;
-            const int token0 = tm * p.bn + (int)rank * own, slot = own * BM;
-            if (own == 2)
+            // the CTA's tokens, half of them for each of the two warps of a quarter
+            const int count = own > 2 ? own / 2 : half == 0 ? own : 0, first = count * half, slot = own * BM;
+            const float *mine = slots + first * BM + row;
+            const int token0 = tm * p.bn + (int)rank * own + first;
+            if (count == 2)
                 finish_joined<2>(p, mine, slot, token0, col, bias);
-            else if (own < 16)
-                for (int t = 0; t < own; t += 4) finish_joined<4>(p, mine + t * BM, slot, token0 + t, col, bias);
-            else if (own < 32)
+            else if (count < 16)
+                for (int t = 0; t < count; t += 4) finish_joined<4>(p, mine + t * BM, slot, token0 + t, col, bias);
+            else if (count < 32)
                 finish_joined<16>(p, mine, slot, token0, col, bias);
             else
-                for (int t = 0; t < own; t += 32) finish_joined<32>(p, mine + t * BM, slot, token0 + t, col, bias);
+                for (int t = 0; t < count; t += 32) finish_joined<32>(p, mine + t * BM, slot, token0 + t, col, bias);
         }
     }
     if (warp == 1) {
