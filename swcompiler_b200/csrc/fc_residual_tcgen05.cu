@@ -314,11 +314,13 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// Up to four tokens.  Reading the weights is all there is to it (a multiply-add per weight and token), and at these sizes a call is
+// One or two tokens.  Reading the weights is all there is to it (a multiply-add per weight and token), and at these sizes a call is
 // a few microseconds, of which a tensor-core kernel's set-up and drain would be half: here every thread requests its whole share of
-// 8 (4 tokens: 4) weight rows at once, multiplies on the FP32 pipe, and the CTA adds up.
+// 8 (two tokens: 4) weight rows at once, multiplies on the FP32 pipe, and the CTA adds up.  4096 x 4096: 7.5 and 8.4 us, 0.69 of
+// the bytes' rate at one token (a tensor-core tile 10 us); 8192 x 8192 at one token 23.6 us, 0.87.  From three tokens on the
+// registers that hold them cost more loads in flight than the tensor cores' set-up (four tokens: 11.1 us against 9.9).
 constexpr int kFewThreads = 256;
-__host__ __device__ constexpr int few_rows(int tokens) { return tokens > 2 ? 4 : 8; }
+__host__ __device__ constexpr int few_rows(int tokens) { return tokens > 1 ? 4 : 8; }
 
 // sums of kV values over the 32 lanes: lane l ends up with the sum of value l % kV
 template <int kV> __device__ __forceinline__ float lanes_sum(float (&v)[kV], int lane) {
@@ -346,7 +348,7 @@ __device__ __noinline__ uint4 load_end(const __nv_bfloat16 *p, int count) {
 }
 
 template <int kTokens>
-__global__ void __launch_bounds__(kFewThreads) fc_res_few_kernel(const __nv_bfloat16 *__restrict__ a, size_t lda,
+__global__ void __launch_bounds__(kFewThreads, kTokens == 1 ? 4 : 1) fc_res_few_kernel(const __nv_bfloat16 *__restrict__ a, size_t lda,
                                                                  const __nv_bfloat16 *__restrict__ w, size_t ldw, const FcrParams p) {
     constexpr int kFewRows = few_rows(kTokens), kV = kFewRows * kTokens;
     __shared__ float part[kFewThreads / 32][kV];
@@ -639,8 +641,8 @@ SWC_EXPORT int swcb200_fc_bf16_residual(swcb200_ctx *ctx, int m, int n, int k, c
     const int sms = swc_tc_sms(ctx);
     CUtensorMap tmW, tmA;
 
-    if (m <= 4) {  // 8.3 us against 10.2 at one token, 4096 x 4096
-        const auto kernel = m == 1 ? fc_res_few_kernel<1> : m == 2 ? fc_res_few_kernel<2> : fc_res_few_kernel<4>;
+    if (m <= 2) {
+        const auto kernel = m == 1 ? fc_res_few_kernel<1> : fc_res_few_kernel<2>;
         SWC_CUDA(ctx, swc_launch_early(kernel, (unsigned)((n + few_rows(m) - 1) / few_rows(m)), kFewThreads, 0, ctx->stream, 1,
                                        (const __nv_bfloat16 *)a_bf16, (size_t)lda, (const __nv_bfloat16 *)wp_bf16, (size_t)ldw, p));
         return swc_check_launch(ctx, "fc_bf16_residual");
