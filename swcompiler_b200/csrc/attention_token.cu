@@ -101,17 +101,21 @@ __device__ __forceinline__ bool find_item(const Params &p, const Known &known, i
     } else if (p.batch <= 32 || !find_seq(p, it.index, [&](const Seq &s) { return items_of(p, s); }, it.seq, i)) {
         return false;
     }
+    int part = 0;
     if (row_tiles(p, it.seq) == 1) {
         it.t0 = 0;
-        it.k0 = i * p.part;
         it.partial = it.seq.nk > p.part;
+        // pieces of one size, so that the CTAs' shares differ little: n of them cover the keys in whole blocks, none above p.part
+        const int n = (it.seq.nk + p.part - 1) / p.part;
+        part = it.partial ? ((it.seq.nk + n - 1) / n + kKeys - 1) / kKeys * kKeys : p.part;
+        it.k0 = i * part;
     } else {
         it.t0 = i * p.tokens;
         it.k0 = 0;
         it.partial = false;
     }
     const int sees = visible(p, it.seq, min(it.t0 + p.tokens, it.seq.nq) - 1);  // the last row sees the most
-    it.k1 = it.partial ? min(it.k0 + p.part, sees) : sees;
+    it.k1 = it.partial ? min(it.k0 + part, sees) : sees;
     return true;
 }
 
@@ -126,7 +130,8 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * kStage);
     uint64_t *empty = full + kStages;
-    uint64_t *item_full = empty + kStages;  // [2] an item's description and query rows are there
+    uint64_t *item_known = empty + kStages;  // [2] an item's description is there
+    uint64_t *item_full = item_known + 2;    // [2] its query rows as well
     uint64_t *item_empty = item_full + 2;
     uint8_t *q_tiles = smem + kStages * kStage + 512;
     // merging: two slots per row group, 16 rows of kD outputs, then the maximum and the sum
@@ -141,6 +146,7 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             mbar_init(&empty[s], kWarps);
         }
         for (int s = 0; s < 2; s++) {
+            mbar_init(&item_known[s], 1);
             mbar_init(&item_full[s], 1);
             mbar_init(&item_empty[s], kWarps + 1);
         }
@@ -161,8 +167,8 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     };
     bool ok = true;
     Item it;
-    const auto next_item = [&] {  // false: no more, or a wait ran out
-        ok = warp_wait(&item_full[items & 1], (items >> 1) & 1, p.status, kWaitFull);
+    const auto next_item = [&](uint64_t *there) {  // false: no more, or a wait ran out
+        ok = warp_wait(&there[items & 1], (items >> 1) & 1, p.status, kWaitFull);
         if (ok) it = s_items[items & 1];
         return ok && it.unit >= 0;
     };
@@ -174,7 +180,10 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             if (!any) it.unit = -1;
             ok = warp_wait(&item_empty[items & 1], ((items >> 1) & 1) ^ 1, p.status, kWaitEmpty);
             if (!ok) break;
-            if (lane == 0) s_items[items & 1] = it;
+            if (lane == 0) {
+                s_items[items & 1] = it;
+                mbar_arrive(&item_known[items & 1]);
+            }
             if (any) {
                 // query rows, 16 bytes at a time; rows of nobody and columns past the width are zeros
                 uint8_t *tile = q_tiles + (items & 1) * Sh::kQTile;
@@ -195,7 +204,7 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         }
     } else if (warp == kWarps) {
         // ------------------------------------------------------------ loads
-        for (; ok && next_item(); items++) {
+        for (; ok && next_item(item_known); items++) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[items & 1]);
             const int head_k = it.unit * p.pack / p.group;
@@ -219,7 +228,7 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const int k_row = kg * 16 + (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;   // K: (keys 0-7: d 0-7, 8-15), (keys 8-15: ..)
         const int v_row = kg * 16 + (lane & 15), v_piece = lane >> 4;                            // V: (keys 0-7, 8-15: d 0-7), (.. d 8-15)
         const int q_row = rg * 16 + (lane & 15), q_piece = lane >> 4;                            // Q: (rows 0-7, 8-15: d 0-7), (.. d 8-15)
-        for (; ok && next_item(); items++) {
+        for (; ok && next_item(item_full); items++) {
             // query fragments, rows g and g + 8 of this row group
             uint32_t qf[kD / 16][4];
             const uint32_t sq = smem_u32(q_tiles + (items & 1) * Sh::kQTile) + q_row * Sh::kQPitch + q_piece * 16;
@@ -396,7 +405,7 @@ constexpr int kJoinThreads = 256;
 template <bool kItems, int kWarps>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Params p, int rows, int parts) {
     constexpr int kRowsPerCta = kJoinThreads / 32 / kWarps;
-    __shared__ float s_o[kWarps > 1 ? kWarps : 1][128], s_l[kWarps];
+    __shared__ float s_o[kWarps > 1 ? kWarps : 1][128], s_l[kWarps], s_m[kWarps];
     const int warp = kWarps > 1 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31;
     const long long which = (long long)blockIdx.x * kRowsPerCta + (kWarps > 1 ? 0 : threadIdx.x >> 5);
     swc_let_next_start();
@@ -445,24 +454,29 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Para
         slot = (size_t)token * p.heads_q + head;
         step = (size_t)p.total_q * p.heads_q;
     }
-    // this warp's parts are warp, warp + kWarps, ...; several of them are read at once
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_lse[slot + i * step]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    // This warp's parts are warp, warp + kWarps, ...: several at once, their sums (a part per lane) and outputs requested together,
+    // with a running maximum.
+    float m = -INFINITY, acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
     const int c = lane * 4;
     constexpr int kAtOnce = kWarps > 1 ? 16 : 8;
     for (int first = warp; first < n; first += kWarps * kAtOnce) {
-        const int mine = first + lane * kWarps;  // the first lanes: the weight of a part each
-        const float w_mine = lane < kAtOnce && mine < n ? exp2_fast(p.part_lse[slot + mine * step] - base) : 0.f;
+        const int mine = first + lane * kWarps;
+        const float lse = lane < kAtOnce && mine < n ? p.part_lse[slot + mine * step] : -INFINITY;
         float4 v[kAtOnce];
 #pragma unroll
         for (int k = 0; k < kAtOnce; k++) {
             const int i = first + k * kWarps;
             v[k] = i < n && c < p.d ? *reinterpret_cast<const float4 *>(p.part_o + (slot + i * step) * p.d + c) : make_float4(0, 0, 0, 0);
         }
+        float top = lse;
+#pragma unroll
+        for (int o = kAtOnce / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(m, __shfl_sync(0xffffffffu, top, 0));
+        const float base = top == -INFINITY ? 0.f : top, factor = exp2_fast(m - base), w_mine = exp2_fast(lse - base);
+        m = top;
+        l *= factor;
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] *= factor;
 #pragma unroll
         for (int k = 0; k < kAtOnce; k++) {
             const float w = __shfl_sync(0xffffffffu, w_mine, k);
@@ -475,16 +489,23 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Para
     }
     if (kWarps > 1) {
         *reinterpret_cast<float4 *>(&s_o[warp][c]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (lane == 0) s_l[warp] = l;
+        if (lane == 0) {
+            s_l[warp] = l;
+            s_m[warp] = m;
+        }
         __syncthreads();
         if (warp != 0) return;
         l = 0.f;
         acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+        m = s_m[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) m = fmaxf(m, s_m[w]);
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
             const float4 v = *reinterpret_cast<const float4 *>(&s_o[w][c]);
-            l += s_l[w];
-            acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
+            const float f = exp2_fast(s_m[w] - (m == -INFINITY ? 0.f : m));
+            l = fmaf(s_l[w], f, l);
+            acc[0] = fmaf(v.x, f, acc[0]), acc[1] = fmaf(v.y, f, acc[1]), acc[2] = fmaf(v.z, f, acc[2]), acc[3] = fmaf(v.w, f, acc[3]);
         }
     }
     if (c < p.d) {

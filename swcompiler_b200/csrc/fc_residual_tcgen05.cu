@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
 // ---------------------------------------------------------------------------------------------------------------------------
 // One or two tokens.  Reading the weights is all there is to it (a multiply-add per weight and token), and at these sizes a call is
 // a few microseconds, of which a tensor-core kernel's set-up and drain would be half: here every thread requests its whole share of
-// 8 (two tokens: 4) weight rows at once, multiplies on the FP32 pipe, and the CTA adds up.  4096 x 4096: 7.5 and 8.4 us, 0.69 of
+// 8 (two tokens: 4) weight rows at once, multiplies on the FP32 pipe, and the CTA adds up.  4096 x 4096: 7.5 and 9 us, 0.69 of
 // the bytes' rate at one token (a tensor-core tile 10 us); 8192 x 8192 at one token 23.6 us, 0.87.  From three tokens on the
 // registers that hold them cost more loads in flight than the tensor cores' set-up (four tokens: 11.1 us against 9.9).
 constexpr int kFewThreads = 256;

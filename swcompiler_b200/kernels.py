@@ -128,6 +128,8 @@ class Backend:
         if dtype is None or t.ndim != 2 or t.get_device() != self._index:
             raise ValueError(f"{what}: expected an fp32 or bf16 matrix on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         rows, cols = t.shape
+        if t.is_contiguous():
+            return t.data_ptr(), dtype, cols, rows, cols
         pitch, step = t.stride()
         if rows <= 1:
             pitch = cols
