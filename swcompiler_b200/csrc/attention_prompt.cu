@@ -245,10 +245,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         tmem_relinquish();
     }
     tc_fence_before();
-    __syncthreads();
+    // A block that gave up on a wait has recorded it: blocks that start after that do not wait in their turn.
+    const bool given_up = __syncthreads_or(*reinterpret_cast<const volatile int *>(p.status) != 0);
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     bool failed = false;
+    if (given_up) {
+        if (warp == 12) tmem_dealloc(tmem, 512);
+        return;
+    }
 
     // The items in turn, for every reader alike: slot and phase follow from the count.
     uint32_t items = 0;
@@ -430,7 +435,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 for (int h = 0; h < 2; h++) {
                     const uint32_t t_s = tmem + h * kKeys, t_o = tmem + 256 + h * 128;
                     const uint32_t parity = blocks_done[h] & 1;
-                    if (j > 0 && (j + 2) * kKeys <= now.sees(h) && j + 1 < now.n(h) && dk == CH * 4) {
+                    if (j > 0 && j + 1 < now.n(h) && dk == CH * 4) {
                         blocks_done[h]++;
                         wait(&p_half[h], parity, kWaitTmemEmpty);
                         tc_fence_after();
@@ -438,6 +443,35 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
                             for (int s = 0; s < kKeys / 32; s++)
                                 umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
+                        }
+                        __syncwarp();
+                        if (stage_k < 0) stage_k = take_stage();
+                        const uint32_t dkey = ring_k + stage_k * (kBlock >> 4);
+                        wait(&p_full[h], parity, kWaitTmemEmpty);
+                        tc_fence_after();
+                        if (!failed && elect_one()) {
+#pragma unroll
+                            for (int s = kKeys / 32; s < kKeys / 16; s++)
+                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
+#pragma unroll
+                            for (int s = 0; s < CH * 4; s++) {
+                                const uint32_t off = (s >> 2) * (kChunk >> 4) + (s & 3) * 2;
+                                umma_bf16_words(t_s, q_lo + h * (kBlock >> 4) + off, dkey + off, idesc_bf16_f32(kRows, kKeys), s != 0);
+                            }
+                            umma_commit(&s_full[h]);
+                            if (j + 2 == now.n(h)) umma_commit(&q_empty[h]);
+                        }
+                        __syncwarp();
+                        continue;
+                    }
+                    if (j == 0 && now.n(h) > 1 && dk == CH * 4) {  // the same for an item's first block
+                        blocks_done[h]++;
+                        wait(&o_empty[h], (tiles_o[h]++ & 1) ^ 1, kWaitTmemEmpty);
+                        wait(&p_half[h], parity, kWaitTmemEmpty);
+                        tc_fence_after();
+                        if (!failed && elect_one()) {
+#pragma unroll
+                            for (int s = 0; s < kKeys / 32; s++) umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, s != 0);
                         }
                         __syncwarp();
                         if (stage_k < 0) stage_k = take_stage();
