@@ -9,7 +9,7 @@
 // (t - mean)^2 over the registers (no E[t^2] - mean^2, which cancels).  pre() reads t before it is rounded to sum's type:
 // the value is there, and rounding it first would only add an error to y.
 //
-// Layout: a row belongs to `tpr` threads.  Up to 32 of them (rows of at most 1024 elements) are a part of one warp and the
+// Layout: a row belongs to `tpr` threads.  Up to 32 of them (rows of at most 512 elements, 256 read singly) are a part of one warp and the
 // sums are shuffles; above that the row is a CTA of its own.  A thread holds at most 32 elements of a row.  Rows whose
 // tensors are all aligned move in chunks of 8 elements (16 bytes of bf16, one 32-byte access of fp32); other rows one
 // element per access, neighbouring threads at neighbouring elements.
@@ -197,7 +197,7 @@ __device__ __forceinline__ void store1(void *p, size_t i, bool is16, float v) {
 
 template <int kVec, int kN, bool kCta, int kX, int kR>
 // (up to 16 elements a thread come with 256 threads at most, and four such CTAs keep an SM busier than three)
-__global__ void __launch_bounds__(!kCta ? 128 : kN * kVec <= 16 ? 256 : kMaxThreads, kCta && kN * kVec <= 16 ? 4 : 1)
+__global__ void __launch_bounds__(!kCta ? 128 : kN * kVec <= 16 ? 256 : kMaxThreads, kCta && kVec == 8 && kN <= 2 ? 4 : 1)
 norm_residual_kernel(const RowParams p) {
     swc_let_next_start();
     swc_after_previous();
@@ -216,11 +216,25 @@ norm_residual_kernel(const RowParams p) {
     if (p.post.kind) norm_row<kVec, kN, kCta>(p.post, p, t, tid, red);
 #pragma unroll
     for (int j = 0; j < kN * kVec; j++) t[j] *= p.scale;
-    if (p.gate) {
+    if (p.gate) {  // one row of it serves many: through L1
         const size_t base = p.gate_rows ? (size_t)(row / p.gate_rows) * p.ldg : 0;
-        load_chunks<kVec, kN, 0>(p.gate, base, p.g_how, p.tpr, cols, tid, x);
+        float g[kN * kVec];
+        if (p.g_how == kF32) {
+            vector_chunks<kVec, kN>(reinterpret_cast<const float *>(p.gate) + base, p, tid, g);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kN * kVec; j++) t[j] *= element<kVec, 0>(x[j / kVec], j % kVec, p.g_how);
+            for (int i = 0; i < kN; i++) {
+                const int c = (i * p.tpr + tid) * kVec;
+                const __nv_bfloat16 *src = reinterpret_cast<const __nv_bfloat16 *>(p.gate) + base + c;
+                uint32_t v[4] = {0u, 0u, 0u, 0u};
+                if (kVec == 8 && c < cols) *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(src));
+                if (kVec == 1 && c < cols) v[0] = (uint32_t)__bfloat16_as_ushort(__ldg(src));
+#pragma unroll
+                for (int e = 0; e < kVec; e++) g[i * kVec + e] = __uint_as_float(e & 1 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kN * kVec; j++) t[j] *= g[j];
     }
     if (p.residual) {
 #pragma unroll
@@ -360,7 +374,7 @@ SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, co
     for (const float *v : {p.post.w, p.post.b, p.pre.w, p.pre.b}) vec = vec && swc_aligned16(v);
     const int chunks = vec ? cols / 8 : cols;
     const int most = vec ? 4 : 32;  // chunks per thread: 32 elements
-    if (chunks <= 32 * most) {      // rows inside a warp
+    if (chunks <= (vec ? 64 : 256)) {  // rows inside a warp
         p.tpr = 1;
         while (p.tpr < 32 && p.tpr * (vec ? 1 : 8) < chunks) p.tpr *= 2;
         const int per_cta = 128 / p.tpr;
@@ -368,8 +382,10 @@ SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, co
         const int n = (chunks + p.tpr - 1) / p.tpr;
         SWC_CUDA(ctx, launch<false>(vec, n, grid, 128, ctx->stream, p));
     } else {
-        // 256 threads where a thread can hold its share: 8192 rows of 4096 in 68 us against 78 with 128 and 83 with 512 threads
-        int per = (chunks + 255) / 256;
+        // 256 threads where a thread can hold its share: 8192 rows of 4096 in 68 us against 78 with 128 and 83 with 512 threads;
+        // where there are rows for every SM, 16 elements a thread at least, 8 read singly (fewer warps to add up: 16384 rows of 2048 with both norms 69 -> 56 us)
+        int per = (chunks + 255) / 256, least = rows >= 2 * (size_t)ctx->sm_count ? (vec ? 2 : 8) : 1;
+        per = per < least ? least : per;
         per = per < most ? per : most;
         int threads = (chunks + per - 1) / per;
         threads = (threads + 31) / 32 * 32;
