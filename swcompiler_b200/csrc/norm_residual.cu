@@ -121,18 +121,19 @@ __device__ __forceinline__ void vector8(const float *p, int i, float (&v)[8]) {
     v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+// (cols: 0 for a row past the last one, whose gate row may not exist)
 template <int kVec, int kN>
-__device__ __forceinline__ void vector_chunks(const float *v, const RowParams &p, int tid, float (&out)[kN * kVec]) {
+__device__ __forceinline__ void vector_chunks(const float *v, const RowParams &p, int cols, int tid, float (&out)[kN * kVec]) {
 #pragma unroll
     for (int i = 0; i < kN; i++) {
         const int c = (i * p.tpr + tid) * kVec;
         if constexpr (kVec == 8) {
             float x[8] = {};
-            if (c < p.cols) vector8(v, c, x);
+            if (c < cols) vector8(v, c, x);
 #pragma unroll
             for (int e = 0; e < 8; e++) out[i * 8 + e] = x[e];
         } else {
-            out[i] = c < p.cols ? __ldg(v + c) : 0.f;
+            out[i] = c < cols ? __ldg(v + c) : 0.f;
         }
     }
 }
@@ -178,8 +179,8 @@ __device__ __forceinline__ void norm_row(const NormParams &n, const RowParams &p
     for (int j = 0; j < kN * kVec; j++) q = fmaf(t[j], t[j], q);
     // the vectors come from L1: all of a thread's chunks at once, behind the sum
     float w[kN * kVec], b[kN * kVec];
-    if (n.w) vector_chunks<kVec, kN>(n.w, p, tid, w);
-    if (n.b) vector_chunks<kVec, kN>(n.b, p, tid, b);
+    if (n.w) vector_chunks<kVec, kN>(n.w, p, p.cols, tid, w);
+    if (n.b) vector_chunks<kVec, kN>(n.b, p, p.cols, tid, b);
     const float rstd = 1.0f / sqrtf(row_sum<kCta>(q, p.tpr, red + 32) * p.inv_cols + n.eps);
 #pragma unroll
     for (int j = 0; j < kN * kVec; j++) {
@@ -220,7 +221,7 @@ norm_residual_kernel(const RowParams p) {
         const size_t base = p.gate_rows ? (size_t)(row / p.gate_rows) * p.ldg : 0;
         float g[kN * kVec];
         if (p.g_how == kF32) {
-            vector_chunks<kVec, kN>(reinterpret_cast<const float *>(p.gate) + base, p, tid, g);
+            vector_chunks<kVec, kN>(reinterpret_cast<const float *>(p.gate) + base, p, cols, tid, g);
         } else {
 #pragma unroll
             for (int i = 0; i < kN; i++) {

@@ -210,6 +210,18 @@ def test_norm_residual_pitches_and_places(be, cols):
         assert torch.equal(wx[:, beside], keep_x[:, beside]) and torch.equal(wr[:, beside], keep_r[:, beside])
 
 
+@pytest.mark.parametrize("rows,cols", [(5, 256), (1, 40), (13, 33), (3, 1000)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_residual_gate_per_row(be, rows, cols, dtype):
+    """A gate row for every row, at row counts that leave a CTA's last rows without one; what lies behind the last one may be anything."""
+    rn = gen(rows + cols)
+    x, room = rn(rows, cols, dtype=BF16), torch.full((rows + 8, cols), float("nan"), dtype=dtype, device="cuda")
+    room[:rows] = rn(rows, cols, dtype=dtype)
+    args = dict(residual=rn(rows, cols), post=(swc.NORM_RMS, None, None, 1e-6), gate=room[:rows], gate_rows=1, scale=1.0,
+                pre=(swc.NORM_LAYER, None, None, 1e-6))
+    norm_check(be.norm_residual(x, **args), x, **args)
+
+
 def test_norm_residual_large_mean_and_constant_rows(be):
     """A layer norm of rows far from zero does not lose the variance; of constant rows it is the bias."""
     rn = gen(3)
