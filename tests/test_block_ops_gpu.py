@@ -392,6 +392,27 @@ def test_attention_wrong_offsets_stay_inside(be, new):
     be.sync()
 
 
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_extreme_offsets(be, new):
+    """The least and largest integers as offsets and lengths: sequences of nothing, or up to the tensors' ends."""
+    rn = gen(14)
+    q, k, v = rn(2 * new, 4, 64, dtype=BF16), rn(300, 2, 64, dtype=BF16), rn(300, 2, 64, dtype=BF16)
+    low, high = -(1 << 31), (1 << 31) - 1
+    at = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    want, tol, _, _ = attention64(q[:new], k, v, new, 300, False, 0.125)
+    out = torch.full_like(q, 7)
+    be.attention_bf16(q, k, v, at(0, new, low), at(low, high, low), causal=False, out=out)  # (the second one: no rows)
+    check(out[:new], want, tol)
+    assert (out[new:] == 7).all()
+    out = torch.full_like(q, 7)
+    be.attention_bf16(q, k, v, at(new, low, new), at(200, low, 300), causal=False, out=out)  # no rows; rows 0 .. new, all keys
+    check(out[:new], want, tol)
+    assert (out[new:] == 7).all()
+    out = be.attention_bf16(q, k, v, at(0, new, high), at(0, 300, low), k_lens=at(high, low), causal=False)
+    check(out[:new], want, tol)
+    assert (out[new:] == 0).all()
+
+
 def test_attention_lengths_change_under_a_graph():
     """One captured call, replayed for other lengths; a second graph in flight has a workspace of its own."""
     s = torch.cuda.Stream()
