@@ -41,11 +41,13 @@ int make_plan(swcb200_ctx *ctx, const swcb200_attention *a, Plan &pl) {
         long long part = keys / (2ll * ctx->sm_count);
         if (part > 2048) part = 512;
         part = part > keys / (32ll * ctx->sm_count) ? part : keys / (32ll * ctx->sm_count);
+        part = part < a->total_k ? part : a->total_k;
         pl.part = (int)((part + 63) / 64 * 64);
         if (pl.part < 64) pl.part = 64;
         const long long items = a->total_k / pl.part + a->total_q / pl.tokens + a->batch;  // each sequence rounds up once
         work = items * pl.units;
-        SWC_REQUIRE(ctx, work < 0x7fffffff, SWCB200_ERR_TOO_LARGE, "attention_bf16: too many work items");
+        // (sums over 32 sequences of up to as many items each have to fit 31 bits)
+        SWC_REQUIRE(ctx, work < 0x7fffffff && items < 1 << 25, SWCB200_ERR_TOO_LARGE, "attention_bf16: too many work items");
         pl.max_items = (int)items;
         if (pl.part < a->total_k) slots = work * pl.rows;
     } else {
@@ -57,7 +59,7 @@ int make_plan(swcb200_ctx *ctx, const swcb200_attention *a, Plan &pl) {
         // Too few tiles for the SMs, as with a short chunk behind a long cache: the keys are divided, in parts of 512 at least.
         pl.parts = 1;
         while (pl.parts < 16 && work * pl.parts * 2 <= ctx->sm_count && (long long)a->total_k / a->batch >= pl.parts * 2ll * 512) pl.parts *= 2;
-        SWC_REQUIRE(ctx, work * pl.parts < 0x7fffffff, SWCB200_ERR_TOO_LARGE, "attention_bf16: too many tiles");
+        SWC_REQUIRE(ctx, work * pl.parts < 0x7fffffff && tiles < 1 << 25, SWCB200_ERR_TOO_LARGE, "attention_bf16: too many tiles");
         pl.tiles = (int)tiles;
         if (pl.parts > 1) slots = (long long)pl.parts * a->total_q * a->heads_q;
     }
@@ -71,6 +73,8 @@ int check(swcb200_ctx *ctx, const swcb200_attention *a) {
     SWC_REQUIRE(ctx, a != nullptr, SWCB200_ERR_BAD_ARG, "attention_bf16: null description");
     SWC_REQUIRE(ctx, a->batch >= 0 && a->total_q >= 0 && a->total_k >= 0 && a->heads_q >= 1 && a->heads_kv >= 1 && a->head_dim >= 1,
                 SWCB200_ERR_BAD_ARG, "attention_bf16: bad shape");
+    SWC_REQUIRE(ctx, a->total_q <= 1 << 30 && a->total_k <= 1 << 30 && a->batch <= 1 << 30, SWCB200_ERR_TOO_LARGE,
+                "attention_bf16: more than 2^30 rows or sequences");
     SWC_REQUIRE(ctx, a->heads_q % a->heads_kv == 0, SWCB200_ERR_BAD_SHAPE,
                 "attention_bf16: %d query heads are no multiple of %d key heads", a->heads_q, a->heads_kv);
     SWC_REQUIRE(ctx, a->head_dim % 8 == 0 && a->head_dim <= 128, SWCB200_ERR_UNSUPPORTED,

@@ -423,14 +423,14 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Para
             int count = 0;
             if (base + lane < p.batch) {
                 s = load_seq(p, base + lane);
-                count = items_of(p, s);
+                count = min(items_of(p, s), p.max_items);
             }
             const unsigned hit = __ballot_sync(0xffffffffu, token >= s.q0 && token < s.q0 + s.nq);
             const int src = hit ? __ffs(hit) - 1 : 32;
             int add = lane < src ? count : 0;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
-            before += add;
+            before = min(before + add, p.max_items);  // (sequences that overlap may number more than there is room for)
             if (hit) {
                 found = base + src;
                 seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);

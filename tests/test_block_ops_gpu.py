@@ -413,6 +413,24 @@ def test_attention_extreme_offsets(be, new):
     assert (out[new:] == 0).all()
 
 
+@pytest.mark.parametrize("new", [1, 5])
+def test_attention_sequences_that_overlap_stay_inside(be, new):
+    """Offsets that name the same rows again and again ask for more pieces of work than the workspace has room for; the call after
+    it is not harmed."""
+    rn = gen(15)
+    n = 200 * new
+    q, k, v = rn(n, 8, 64, dtype=BF16), rn(4000, 2, 64, dtype=BF16), rn(4000, 2, 64, dtype=BF16)
+    off = torch.zeros(201, dtype=torch.int32, device="cuda")
+    for rows in (new, n):  # every second sequence has the same rows and all keys
+        off_q, off_k = off.clone(), off.clone()
+        off_q[1::2], off_k[1::2] = rows, 4000
+        be.attention_bf16(q, k, v, off_q, off_k, causal=False)
+    be.sync()
+    got = be.attention_bf16(q[:new], k, v, offsets([new]), offsets([4000]), causal=False)
+    want, tol, _, _ = attention64(q[:new], k, v, new, 4000, False, 0.125)
+    check(got, want, tol)
+
+
 def test_attention_lengths_change_under_a_graph():
     """One captured call, replayed for other lengths; a second graph in flight has a workspace of its own."""
     s = torch.cuda.Stream()
@@ -498,6 +516,9 @@ def test_attention_empty_and_refused(be):
     need = C.c_size_t()
     assert be.lib.swcb200_attention_workspace(be._ctx, K._ATTENTION.pack(*a, 0, 0), C.byref(need)) == L.OK and need.value > 0
     assert be.lib.swcb200_attention_bf16(be._ctx, K._ATTENTION.pack(*a, 0, 0)) == L.ERR_BAD_ARG
+    for i in (13, 14, 15):  # batch, total_q, total_k
+        assert be.lib.swcb200_attention_workspace(be._ctx, K._ATTENTION.pack(*a[:i], (1 << 30) + 1, *a[i + 1:], 0, 0), C.byref(need)) == L.ERR_TOO_LARGE
+    assert be.lib.swcb200_attention_workspace(be._ctx, K._ATTENTION.pack(*a, 0, 0), C.byref(need)) == L.OK
     ws = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
     assert be.lib.swcb200_attention_bf16(be._ctx, K._ATTENTION.pack(*a, ws.data_ptr(), need.value - 1)) == L.ERR_BAD_ARG
     assert be.lib.swcb200_attention_bf16(be._ctx, K._ATTENTION.pack(*a, ws.data_ptr() + 8, need.value)) == L.ERR_MISALIGNED
