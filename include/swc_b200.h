@@ -247,8 +247,8 @@ int swcb200_maxpool_bf16(swcb200_ctx *ctx, const void *input, void *output, cons
  * bf16 under the rules of swcb200_fc_bf16: 16-byte aligned, lda and ldw multiples of 8; C and the
  * residual fp32 or bf16 at any alignment and pitch.  Sums, bias, activation and residual are fp32,
  * rounded once at the store.  The residual may be C itself (same pointer, type and leading
- * dimension), any other overlap of the two is refused.  Any m from one row on: few rows divide k
- * over a cluster of CTAs. */
+ * dimension); any other overlap of C with the residual, A, Wp or the bias is refused.  Any m from one
+ * row on (few rows divide k over a cluster of CTAs); m, n and k up to 2^30. */
 typedef struct swcb200_fc_epilogue {
     const float *bias; /* [n] or NULL */
     int act;           /* enum swcb200_act, all of them */
@@ -275,8 +275,8 @@ typedef struct swcb200_norm {
  * leaves residual, gate or sum out (sum or y has to be there); y and pre go together.  Row r is
  * multiplied by gate row r / gate_rows, or every row by the one gate row where gate_rows is 0.
  * All arithmetic is fp32; t goes into pre() unrounded.  sum and y may each be x or residual in
- * place (same pointer, type and leading dimension), other overlaps are refused.  Rows of one call
- * at any alignment; 128- and 256-bit accesses where all pointers allow them.  cols <= 16384. */
+ * place (same pointer, type and leading dimension), other overlaps are refused, with the norms'
+ * vectors too.  Rows of one call at any alignment; 128- and 256-bit accesses where all pointers allow them.  cols <= 16384. */
 typedef struct swcb200_norm_block {
     const void *x;
     int x_dtype;

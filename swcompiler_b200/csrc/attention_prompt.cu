@@ -270,7 +270,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         return it.valid != 0;
     };
 
-    // registers: 512 x 128 at launch = 256 x 176 for the softmax + 128 x 80 for the output + 128 x 80
+    // registers: 512 x 128 at launch = 256 x 192 for the softmax + 128 x 72 for the output + 128 x 56
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 14) {

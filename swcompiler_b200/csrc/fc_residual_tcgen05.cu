@@ -626,12 +626,20 @@ SWC_EXPORT int swcb200_fc_bf16_residual(swcb200_ctx *ctx, int m, int n, int k, c
     SWC_REQUIRE(ctx, a_bf16 && wp_bf16 && c, SWCB200_ERR_BAD_ARG, "fc_bf16_residual: null tensor");
     SWC_REQUIRE(ctx, swc_aligned16(a_bf16) && swc_aligned16(wp_bf16) && lda % 8 == 0 && ldw % 8 == 0, SWCB200_ERR_MISALIGNED,
                 "fc_bf16_residual: A and Wp start on 16 bytes, lda (%d) and ldw (%d) are multiples of 8 elements", lda, ldw);
+    SWC_REQUIRE(ctx, m <= 1 << 30 && n <= 1 << 30 && k <= 1 << 30, SWCB200_ERR_TOO_LARGE, "fc_bf16_residual: more than 2^30 rows or columns");
     SWC_REQUIRE(ctx, lda >= k && ldw >= k && ldc >= n && (!ep->residual || ep->ld_residual >= n), SWCB200_ERR_BAD_SHAPE,
                 "fc_bf16_residual: leading dimension too small");
     const size_t ce = c_dtype == SWCB200_BF16 ? 2 : 4, re = ep->residual_dtype == SWCB200_BF16 ? 2 : 4;
     SWC_REQUIRE(ctx, !ep->residual || (ep->residual == c && ce == re && (m == 1 || ep->ld_residual == ldc)) ||
                 !swc_rows_overlap(c, ldc * ce, n * ce, ep->residual, ep->ld_residual * re, n * re, (size_t)m),
                 SWCB200_ERR_BAD_ARG, "fc_bf16_residual: C overlaps the residual without being the same tensor");
+    // other CTAs still read A, Wp and the bias when one stores its tile
+    const auto end = [](const void *q, int rows, size_t pitch, size_t width) { return (const char *)q + (size_t)(rows - 1) * pitch + width; };
+    const char *c0 = (const char *)c, *c1 = end(c, m, ldc * ce, n * ce), *w0 = (const char *)wp_bf16;
+    SWC_REQUIRE(ctx, !swc_rows_overlap(c, ldc * ce, n * ce, a_bf16, (size_t)lda * 2, (size_t)k * 2, (size_t)m) &&
+                (c1 <= w0 || end(w0, n, (size_t)ldw * 2, (size_t)k * 2) <= c0) &&
+                (!ep->bias || c1 <= (const char *)ep->bias || (const char *)(ep->bias + n) <= c0),
+                SWCB200_ERR_BAD_ARG, "fc_bf16_residual: C overlaps A, Wp or the bias");
     FcrParams p = {};
     p.m = m, p.n = n, p.k = k;
     p.bias = ep->bias, p.act = ep->act, p.scale = ep->scale;

@@ -342,12 +342,17 @@ SWC_EXPORT int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, co
         const char *a0 = (const char *)a.p, *b0 = (const char *)b.p;
         return a0 < b0 + ((b.rows - 1) * b.ld + c) * b.size && b0 < a0 + ((a.rows - 1) * a.ld + c) * a.size;
     };
-    for (const Tensor &o : out)
+    for (const Tensor &o : out) {
+        for (const swcb200_norm *n : norms)
+            for (const float *v : {n->weight, n->bias})
+                SWC_REQUIRE(ctx, !o.p || !v || n->kind == SWCB200_NORM_NONE || (const char *)o.p + ((rows - 1) * o.ld + c) * o.size <= (const char *)v ||
+                            v + c <= o.p, SWCB200_ERR_BAD_ARG, "norm_residual: an output overlaps a norm's vector");
         for (int i = 0; i < 3; i++) {
             const bool in_place = i < 2 && o.p == in[i].p && o.size == in[i].size && (rows == 1 || o.ld == in[i].ld);
             SWC_REQUIRE(ctx, in_place || !meet(o, in[i]), SWCB200_ERR_BAD_ARG,
                         "norm_residual: an output overlaps an input without being the same tensor");
         }
+    }
     SWC_REQUIRE(ctx, !meet(out[0], out[1]), SWCB200_ERR_BAD_ARG, "norm_residual: the two outputs overlap");
 
     RowParams p = {};

@@ -126,6 +126,22 @@ def test_fc_bf16_residual_empty_and_refused(be):
         be.fc_bf16_residual(a.cpu(), wp)
 
 
+@pytest.mark.parametrize("m", [1, 4, 200])
+def test_fc_bf16_residual_refuses_to_overwrite_its_operands(be, m):
+    a, wide, room = torch.zeros(m, 64, dtype=BF16, device="cuda"), torch.zeros(m, 128, dtype=BF16, device="cuda"), torch.zeros(m * 64 + 64, device="cuda")
+    weights = torch.zeros(64 * 64 + m * 64, dtype=BF16, device="cuda")
+    wp = weights[:64 * 64].view(64, 64)
+    for args in (dict(a=a, out=a), dict(a=wide[:, :64], out=wide[:, 8:72]), dict(a=a, out=weights[64 * 63:64 * (63 + m)].view(m, 64)),
+                 dict(a=a, bias=room[32:96], out=room[:m * 64].view(m, 64))):
+        with pytest.raises(swc.SwcError) as e:
+            be.fc_bf16_residual(wp=wp, **args)
+        assert e.value.status == L.ERR_BAD_ARG
+    # side by side is no overlap
+    be.fc_bf16_residual(wide[:, :64], wp, bias=room[m * 64:], out=wide[:, 64:])
+    be.fc_bf16_residual(a, wp, out=weights[64 * 64:].view(m, 64))
+    be.fc_bf16_residual(a, wp, bias=room[m * 64:], out=room[:m * 64].view(m, 64))
+
+
 # ------------------------------------------------------------------ norm_residual
 
 def norm64(t, tol, norm):
@@ -208,6 +224,17 @@ def test_norm_residual_pitches_and_places(be, cols):
         beside = torch.ones(cols + 24, dtype=torch.bool, device="cuda")
         beside[shift:shift + cols] = False
         assert torch.equal(wx[:, beside], keep_x[:, beside]) and torch.equal(wr[:, beside], keep_r[:, beside])
+
+
+def test_norm_residual_refuses_to_overwrite_its_vectors(be):
+    room = torch.zeros(5 * 64, device="cuda")
+    x, w = torch.zeros(4, 64, device="cuda"), room[4 * 64 - 8:5 * 64 - 8]
+    for norm in ((swc.NORM_LAYER, w, None, 1e-6), (swc.NORM_RMS, None, w, 1e-6)):
+        for args in (dict(pre=norm, y=room[:256].view(4, 64)), dict(pre=norm, sum=room[:256].view(4, 64)), dict(post=norm, sum=room[:256].view(4, 64))):
+            with pytest.raises(swc.SwcError) as e:
+                be.norm_residual(x, **args)
+            assert e.value.status == L.ERR_BAD_ARG
+    be.norm_residual(x, pre=(swc.NORM_RMS, room[256:], None, 1e-6), y_dtype=F32, sum=room[:256].view(4, 64))  # behind it is no overlap
 
 
 @pytest.mark.parametrize("rows,cols", [(5, 256), (1, 40), (13, 33), (3, 1000)])
