@@ -1,4 +1,4 @@
-"""Per-kernel roofline measurements on one GPU:  python -m swcompiler_b200.opbench [--only NAME] [--iters N]
+"""Per-kernel roofline measurements on one GPU:  python -m swcompiler_b200.opbench [--only NAME] [--iters N] [--blocks | --latency]
 
 Times every kernel of the table at the sizes the benchmark configurations give it (config 5 stage
 [256,56,56,64], config 3 activations [65536,4096] and logits [65536,1000]), with CUDA events on the
@@ -234,16 +234,63 @@ def op_rows(iters=20, only=None):
     return rows
 
 
+def block_rows(iters=20, only=None):
+    """One row per kernel of the transformer-block calls: the calls whose own time is longer than the host's."""
+    hbm, tflops, src = _peaks()
+    be = swc.Backend(torch.cuda.current_device(), swc.TC_BF16)
+    dev = be.device
+    g = torch.Generator(device=dev).manual_seed(0)
+    rn = lambda *shape, dtype=torch.bfloat16: torch.randn(shape, generator=g, device=dev).to(dtype)
+    at = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    rows = []
+
+    def row(name, fn, nbytes=0, flops=0):
+        if only and only not in name:
+            return
+        t = _time(fn, iters, rest=1.0 if flops else 0.0)
+        bound = dict(bound="tensor", achieved=flops / t / 1e12, unit="TFLOP/s", peak=tflops, frac=flops / t / 1e12 / tflops, flops=flops,
+                     peak_source=src + " (burst)") if flops else dict(bound="hbm", achieved=nbytes / t / 1e9, unit="GB/s", peak=hbm,
+                                                                      frac=nbytes / t / 1e9 / hbm, bytes=nbytes, peak_source=src)
+        rows.append({"kernel": name, "us": t * 1e6, **bound})
+
+    d = 4096
+    rms, layer = (swc.NORM_RMS, rn(d, dtype=torch.float32), None, 1e-6), (swc.NORM_LAYER, rn(d, dtype=torch.float32), rn(d, dtype=torch.float32), 1e-5)
+    x, r = rn(8192, d), rn(8192, d)
+    t, y = torch.empty_like(x), torch.empty_like(x)
+    row("norm_residual [8192,4096] rms both sides", lambda: be.norm_residual(x, residual=r, post=rms, pre=rms, sum=t, y=y), nbytes=8 * x.numel())
+    x, r, gate = rn(65536, d), rn(65536, d, dtype=torch.float32), rn(1, d, dtype=torch.float32)
+    t, y = torch.empty_like(r), torch.empty_like(x)
+    row("norm_residual [65536,4096] gate, fp32 sum, layer norm", lambda: be.norm_residual(x, residual=r, gate=gate, pre=layer, sum=t, y=y),
+        nbytes=12 * x.numel())
+    del r, t, y
+    m = 16384
+    a, wp, b, r, c = x[:m], rn(d, d), rn(d, dtype=torch.float32), rn(m, d), torch.empty(m, d, dtype=torch.bfloat16, device=dev)
+    row("fc_bf16_residual 16384x4096x4096 +bias+gelu+residual",
+        lambda: be.fc_bf16_residual(a, wp, b, swc.ACT_GELU_TANH, residual=r, out=c), flops=2.0 * m * d * d)
+    q, k, v, off = rn(m, 16, 128), rn(m, 4, 128), rn(m, 4, 128), at(0, m)
+    o = torch.empty_like(q)
+    row("attention_bf16 16384 tokens, 16 heads, 4 key heads of 128, causal", lambda: be.attention_bf16(q, k, v, off, off, out=o),
+        flops=2.0 * m * (m + 1) * 16 * 128)
+    for batch, n in ((1, 65536), (64, 4096)):
+        q1, k1, v1 = rn(batch, 32, 128), rn(batch * n, 8, 128), rn(batch * n, 8, 128)
+        o1, off_q, off_k = torch.empty_like(q1), at(*range(batch + 1)), at(*range(0, batch * n + 1, n))
+        row(f"attention_bf16 one token each, {batch} caches of {n} keys, 32 heads, 8 key heads of 128",
+            lambda: be.attention_bf16(q1, k1, v1, off_q, off_k, out=o1), nbytes=4 * k1.numel())
+    be.sync()
+    return rows
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--only", default=None)
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--latency", action="store_true",
                     help="the two small configurations (MLP batch 64, LeNet-style net batch 32): microseconds per forward")
+    ap.add_argument("--blocks", action="store_true", help="the transformer-block calls")
     args = ap.parse_args()
     if args.latency:
         return latency(args.iters)
-    for r in op_rows(args.iters, args.only):
+    for r in (block_rows if args.blocks else op_rows)(args.iters, args.only):
         print(json.dumps(r))
 
 

@@ -590,3 +590,52 @@ def test_a_block_of_a_transformer(be, decode):
     t, y = be.norm_residual(down, residual=stream, post=norm1, scale=0.5, pre=norm2, sum=stream)  # the next block's way in
     norm_check((t, y), down, before, norm1, None, 0, 0.5, norm2)
     be.sync()
+
+
+def test_two_streams_with_captured_blocks_at_once():
+    """The same chain eager, and captured by two contexts whose graphs are replayed side by side, again and again: the same bits."""
+    hq, hkv, d, width = 8, 2, 128, 1024
+    norm = (swc.NORM_RMS, None, None, 1e-6)
+
+    def block(be, x, w_qkv, w_o, q_off, k_off, cache_k, cache_v, n):
+        _, h = be.norm_residual(x, pre=norm, want_sum=False)
+        qkv = be.fc_bf16_residual(h, w_qkv)
+        q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((hq * d, hkv * d, hkv * d), 1))
+        whole = be.attention_bf16(q, k, v, q_off, q_off)                          # the rows as prompts
+        cached = be.attention_bf16(q[:n], cache_k, cache_v, k_off[0], k_off[1])   # the first ones as new tokens over a cache
+        x2 = be.fc_bf16_residual(whole.flatten(1), w_o, residual=x, out_dtype=F32)
+        x3 = be.fc_bf16_residual(cached.flatten(1), w_o, act=swc.ACT_SILU)
+        return be.norm_residual(x2, pre=norm) + (x3,)
+
+    cases = []
+    for i, (lengths, n) in enumerate((([300, 5, 170], 3), ([64, 700], 1))):
+        rn = gen(30 + i)
+        rows = sum(lengths)
+        cases.append((rn(rows, width), rn((hq + 2 * hkv) * d, width, dtype=BF16, s=0.03), rn(width, hq * d, dtype=BF16, s=0.03), offsets(lengths),
+                      (offsets([1] * n), offsets([2500] * n)), rn(2500 * n, hkv, d, dtype=BF16), rn(2500 * n, hkv, d, dtype=BF16), n))
+    be = swc.Backend(0, swc.TC_BF16)
+    want = [[t.clone() for t in block(be, *c)] for c in cases]
+    torch.cuda.synchronize()
+    lanes = []
+    for c in cases:
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            lane = swc.Backend(0, swc.TC_BF16, stream=s)
+            block(lane, *c)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                out = block(lane, *c)
+        lanes.append((s, lane, g, out))
+    for _ in range(5):
+        for s, _, g, out in lanes:
+            with torch.cuda.stream(s):
+                for t in out:
+                    t.zero_()
+                g.replay()
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, lane, _, out), expect in zip(lanes, want):
+        lane.sync()
+        for got, ref in zip(out, expect):
+            assert torch.equal(got, ref)
