@@ -20,8 +20,12 @@
 // per cycle), but the two tiles together take some 3200 cycles per block: a tile's softmax (1900) and the products between two
 // of them (1030) are a chain, as there is room for one block of scores per tile.  At width 128 and long prompts that is also
 // where the power limit sets the clock: 16 heads, 4 key heads, 16384 keys, causal: 855 us, 1290 TFLOP/s, 0.80 of the burst and
-// 0.96 of the sustained bf16 rate measured here; width 64: 800 us.  Prompts of a few hundred tokens spend as long at the items'
-// ends (first scores, last output) as in between: 64 sequences of 197, 16 heads of 64: 57 us, a quarter of the bytes' rate.
+// 0.96 of the sustained bf16 rate measured here; width 64: 771 us.  Prompts of a few hundred tokens spend as long at the items'
+// ends as in between: 64 sequences of 197, 16 heads of 64: 55 us, 0.29 of the bytes' rate.  There the softmax runs its first and
+// masked blocks, whose code the warps do not have at hand (a fifth of their time goes to waiting for instructions; a block takes
+// 2600 to 5200 cycles instead of 1900), while the output warps turn the item before around.  So what nobody needs is left out:
+// tiles without rows, warps whose rows are nobody's, the last quarter of a block that is seen half (64 sequences of 128 keys of
+// width 64: 38 -> 31 us; 64 of 256, 32 heads of 128: 122 -> 116 us).
 // Measured and not kept: scores of blocks of 64 keys two ahead (the instructions around twice as many blocks cost what the chain
 // does), an issuing warp per tile (the tiles fall into step: 1088 us).
 #include "attention_common.cuh"
@@ -546,6 +550,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 const float2 stat = s_stat[h][row];
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&stat_empty[h]);
+                if (first >= it.seq.nq) continue;  // no rows, and n is 0
                 if (!failed && n > 0 && !warp_wait(&o_full[h], tiles_done[h]++ & 1, p.status, kWaitTmemFull)) failed = true;
                 if (failed) break;
                 tc_fence_after();
@@ -626,6 +631,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             const int sees = visible(p, it.seq, min(t, it.seq.nq - 1)) - it.j0 * kKeys;  // keys of this part that the row sees,
             const int all_see = visible(p, it.seq, first) - it.j0 * kKeys;              // that every row of the tile sees,
             const int one_sees = it.sees(h);                                            // that some row of it sees
+            const bool idle = !__any_sync(0xffffffffu, tok < p.tokens && t < it.seq.nq);  // no row of this warp is anybody's
             float m = -INFINITY;                                // the maximum that the weights are relative to (raw scores)
             uint64_t l = pair(0.f, 0.f);    // the weights' sum
             for (int j = 0; j < n; j++) {
@@ -643,6 +649,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar);
                 };
+                if (idle) {
+                    publish(&p_half[h]);
+                    publish(&p_full[h]);
+                    continue;
+                }
                 // a maximum that has grown: sums and output are brought to it
                 const auto grow = [&](float top) {
                     float factor = 1.f;
@@ -673,7 +684,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 tmem_ld_wait();
                 if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < kKeys; c++) s[c] = c < mine ? s[c] : -INFINITY;
+                    for (int c0 = 0; c0 < kKeys; c0 += 32) {
+                        const int left = mine - c0;
+                        const uint32_t seen = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1 : 0u;
+#pragma unroll
+                        for (int c = 0; c < 32; c++) s[c0 + c] = seen & (1u << c) ? s[c0 + c] : -INFINITY;
+                    }
                 }
                 if (j == 0) grow(largest<kKeys>(s));
                 // The first half's weights are taken relative to the maximum so far, while this block's is looked for: that is off the
@@ -695,7 +711,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 if (keys > 64) {  // (weights of keys that no row of the tile sees are not multiplied either)
                     const uint64_t b = base();
                     weights(s + 64, scale2, b, t_s + 32, l);
-                    weights(s + 96, scale2, b, t_s + 48, l);
+                    if (keys > 96) weights(s + 96, scale2, b, t_s + 48, l);
                 }
                 publish(&p_full[h]);
             }
