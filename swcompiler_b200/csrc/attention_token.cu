@@ -10,6 +10,9 @@
 // With 16 rows the tensor cores are a side matter (a 128-row tcgen05 tile would be seven eighths padding), so each warp runs
 // mma.sync m16n8k16 on 16 of a block's 64 keys with a softmax of its own in registers -- no barrier between warps until the end
 // of an item, where the four key groups are merged.
+//
+// 32 heads, 8 key heads of 128, one token each: 64 caches of 4096 keys 173 us, 0.95 of the copy rate measured here; 64 ragged ones of up
+// to 4096 keys 64 us, 0.79 (CTAs that end apart); one cache of 65536 keys 50 us with its join, 0.82.
 #include "attention_common.cuh"
 
 namespace {

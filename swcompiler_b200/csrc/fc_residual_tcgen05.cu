@@ -12,7 +12,8 @@
 //   through distributed shared memory in rank order, no workspace, the same result on every run.  For calls whose tiles alone
 //   would leave SMs idle; with few tokens it is bound by reading Wp once.
 // fc_res_pair_kernel: persistent CTA pairs (cta_group::2), 256 x BN tiles, two accumulators so that the epilogue of a tile runs
-//   beside the main loop of the next.  For everything else; bound by the tensor pipe.
+//   beside the main loop of the next.  For everything else; bound by the tensor pipe: 16384 x 4096 x 4096 with bias, tanh-GELU and a
+//   bf16 residual 378 us, 1455 TFLOP/s, 0.91 of the burst rate of a library product measured here.
 #include "tc_common.cuh"
 
 namespace {
@@ -593,8 +594,9 @@ struct Choice {
 // The form with the least time by a model of it: waves over the SMs, times what a CTA spends on its k blocks and beside them.
 // Measured at k = 4096, in us: a 64-deep block takes 0.11 / 0.12 / 0.155 / 0.19 / 0.28 at 16 / 32 / 64 / 128 / 256 tokens (the
 // issuing threads, then loads), 0.30 in the pair form (the tensor pipe at 256 x 256); launch, first loads, epilogue 6.5 + 0.016 per
-// token; the join over 2 / 4 / 8 CTAs 0.8 / 2 / 3.5.  (m, n) = (777, 1000): chosen 128 tokens over 2 CTAs 14.7 us; 4 CTAs (two
-// waves) 21.6; undivided 19.9; 256 tokens over 4 18.1; pairs 26.1.  (64, 4096): 64 over 4 11.1; over 8 12.4; undivided 17.7.
+// token; the join over 2 / 4 / 8 CTAs 0.8 / 2 / 3.5.  Forms compared in one run, (m, n) = (777, 1000): chosen 128 tokens over 2
+// CTAs 14.7 us; 4 CTAs (two waves) 21.6; undivided 19.9; 256 tokens over 4 18.1; pairs 26.1.  (64, 4096): 64 over 4 11.1; over 8
+// 12.4; undivided 17.7.
 Choice choose(int m, int n, int kblocks, int sms) {
     Choice best = {true, BN_MAX, 1};
     const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
