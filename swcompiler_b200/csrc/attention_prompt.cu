@@ -21,13 +21,14 @@
 // of them (1030) are a chain, as there is room for one block of scores per tile.  At width 128 and long prompts that is also
 // where the power limit sets the clock: 16 heads, 4 key heads, 16384 keys, causal: 855 us, 1290 TFLOP/s, 0.80 of the burst and
 // 0.96 of the sustained bf16 rate measured here; width 64: 771 us.  Prompts of a few hundred tokens spend as long at the items'
-// ends as in between: 64 sequences of 197, 16 heads of 64: 55 us, 0.29 of the bytes' rate.  There the softmax runs its first and
+// ends as in between: 64 sequences of 197, 16 heads of 64: 53 to 60 us, 0.28 of the bytes' rate.  There the softmax runs its first and
 // masked blocks, whose code the warps do not have at hand (a fifth of their time goes to waiting for instructions; a block takes
-// 2600 to 5200 cycles instead of 1900), while the output warps turn the item before around.  So what nobody needs is left out:
-// tiles without rows, warps whose rows are nobody's, the last quarter of a block that is seen half (64 sequences of 128 keys of
-// width 64: 38 -> 31 us; 64 of 256, 32 heads of 128: 122 -> 116 us).
+// 2600 to 5200 cycles instead of 1900), while the output warps turn the item before around.  So what nobody needs is left out
+// (tiles without rows, warps whose rows are nobody's, the last quarter of a block that is seen half: 64 sequences of 128 keys of
+// width 64, 38 -> 31 us), and code is shared where that costs the long prompts nothing (-> 29 us).
 // Measured and not kept: scores of blocks of 64 keys two ahead (the instructions around twice as many blocks cost what the chain
-// does), an issuing warp per tile (the tiles fall into step: 1088 us).
+// does), an issuing warp per tile (the tiles fall into step: 1088 us), the loop over the two tiles rolled in the issuing warp, or an
+// item's first block in the loop of the others (50 to 56 us for the 64 sequences of 197, but 885 and 878 for 16384 keys).
 #include "attention_common.cuh"
 
 namespace {
@@ -439,43 +440,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 for (int h = 0; h < 2; h++) {
                     const uint32_t t_s = tmem + h * kKeys, t_o = tmem + 256 + h * 128;
                     const uint32_t parity = blocks_done[h] & 1;
-                    if (j > 0 && j + 1 < now.n(h) && dk == CH * 4) {
+                    if (j + 1 < now.n(h) && dk == CH * 4) {
                         blocks_done[h]++;
+                        if (j == 0) wait(&o_empty[h], (tiles_o[h]++ & 1) ^ 1, kWaitTmemEmpty);
                         wait(&p_half[h], parity, kWaitTmemEmpty);
                         tc_fence_after();
-                        if (elect_one()) {
+                        if (!failed && elect_one()) {
 #pragma unroll
                             for (int s = 0; s < kKeys / 32; s++)
-                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
-                        }
-                        __syncwarp();
-                        if (stage_k < 0) stage_k = take_stage();
-                        const uint32_t dkey = ring_k + stage_k * (kBlock >> 4);
-                        wait(&p_full[h], parity, kWaitTmemEmpty);
-                        tc_fence_after();
-                        if (!failed && elect_one()) {
-#pragma unroll
-                            for (int s = kKeys / 32; s < kKeys / 16; s++)
-                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, true);
-#pragma unroll
-                            for (int s = 0; s < CH * 4; s++) {
-                                const uint32_t off = (s >> 2) * (kChunk >> 4) + (s & 3) * 2;
-                                umma_bf16_words(t_s, q_lo + h * (kBlock >> 4) + off, dkey + off, idesc_bf16_f32(kRows, kKeys), s != 0);
-                            }
-                            umma_commit(&s_full[h]);
-                            if (j + 2 == now.n(h)) umma_commit(&q_empty[h]);
-                        }
-                        __syncwarp();
-                        continue;
-                    }
-                    if (j == 0 && now.n(h) > 1 && dk == CH * 4) {  // the same for an item's first block
-                        blocks_done[h]++;
-                        wait(&o_empty[h], (tiles_o[h]++ & 1) ^ 1, kWaitTmemEmpty);
-                        wait(&p_half[h], parity, kWaitTmemEmpty);
-                        tc_fence_after();
-                        if (!failed && elect_one()) {
-#pragma unroll
-                            for (int s = 0; s < kKeys / 32; s++) umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, s != 0);
+                                umma_output(t_o, t_s + s * 8, dv + s * (16 * 128 >> 4), idesc_o, s != 0 || j != 0);
                         }
                         __syncwarp();
                         if (stage_k < 0) stage_k = take_stage();
@@ -539,10 +512,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const int tok = row * p.pack_inv >> 16, head_in = row - tok * p.pack;
         uint8_t *patch = patches + quarter * kPatch;
-        uint32_t tiles_done[2] = {0, 0}, items_done = 0;
+        uint32_t tiles_done = 0, items_done = 0;  // tiles_done: a bit per tile
         Item it;
         while (!failed && next_item(it)) {
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < 2; h++) {
                 const int n = it.n(h), first = it.t0 + h * p.tokens;
                 const uint32_t t_o = tmem + ((uint32_t)(quarter * 32) << 16) + 256 + h * 128;
@@ -551,8 +524,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&stat_empty[h]);
                 if (first >= it.seq.nq) continue;  // no rows, and n is 0
-                if (!failed && n > 0 && !warp_wait(&o_full[h], tiles_done[h]++ & 1, p.status, kWaitTmemFull)) failed = true;
+                if (!failed && n > 0 && !warp_wait(&o_full[h], tiles_done >> h & 1, p.status, kWaitTmemFull)) failed = true;
                 if (failed) break;
+                if (n > 0) tiles_done ^= 1u << h;
                 tc_fence_after();
                 const bool empty_row = stat.x == 0.f;  // nothing seen
                 const float inv = 1.f / stat.x;
