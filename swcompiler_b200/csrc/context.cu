@@ -50,15 +50,17 @@ static int init_common(int device, int precision, void *stream, bool own, swcb20
         return SWCB200_ERR_NO_DEVICE;
     }
     if (device < 0 || device >= count) return SWCB200_ERR_BAD_ARG;
-    cudaDeviceProp prop;
-    if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) return SWCB200_ERR_CUDA;
+    int major = 0, sms = 0;  // (two attributes: asking for all properties takes milliseconds)
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+        return SWCB200_ERR_CUDA;
     // the library holds sm_100a code only
-    if (prop.major != 10) return SWCB200_ERR_NO_DEVICE;
+    if (major != 10) return SWCB200_ERR_NO_DEVICE;
     if (cudaSetDevice(device) != cudaSuccess) return SWCB200_ERR_CUDA;
     swcb200_ctx *ctx = new swcb200_ctx();
     ctx->device = device;
     ctx->precision = precision;
-    ctx->sm_count = prop.multiProcessorCount;
+    ctx->sm_count = sms;
     if (own) {
         if (cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess) {
             delete ctx;
