@@ -21,14 +21,14 @@
 // of them (1030) are a chain, as there is room for one block of scores per tile.  At width 128 and long prompts that is also
 // where the power limit sets the clock: 16 heads, 4 key heads, 16384 keys, causal: 855 us, 1290 TFLOP/s, 0.80 of the burst and
 // 0.96 of the sustained bf16 rate measured here; width 64: 771 us.  Prompts of a few hundred tokens spend as long at the items'
-// ends as in between: 64 sequences of 197, 16 heads of 64: 53 to 60 us, 0.28 of the bytes' rate.  There the softmax runs its first and
-// masked blocks, whose code the warps do not have at hand (a fifth of their time goes to waiting for instructions; a block takes
-// 2600 to 5200 cycles instead of 1900), while the output warps turn the item before around.  So what nobody needs is left out
-// (tiles without rows, warps whose rows are nobody's, the last quarter of a block that is seen half: 64 sequences of 128 keys of
-// width 64, 38 -> 31 us), and code is shared where that costs the long prompts nothing (-> 29 us).
+// ends as in between: 64 sequences of 197, 16 heads of 64: 46 us, 0.35 of the bytes' rate.  There the softmax runs its first and
+// masked blocks, whose code the warps do not have at hand (a fifth of their time went to waiting for instructions; a block took 2600
+// to 5200 cycles instead of 1900), while the output warps turn the item before around.  So what nobody needs is left out (tiles
+// without rows, warps whose rows are nobody's, the last quarter of a block that is seen half: 64 sequences of 128 keys of width 64,
+// 38 -> 31 us), and there is less code: the output warps' loop over the two tiles is rolled, and in the form for short prompts
+// (kShort) also that of the issuing warp, and an item's first block goes through the loop of the others (-> 27 us).
 // Measured and not kept: scores of blocks of 64 keys two ahead (the instructions around twice as many blocks cost what the chain
-// does), an issuing warp per tile (the tiles fall into step: 1088 us), the loop over the two tiles rolled in the issuing warp, or an
-// item's first block in the loop of the others (50 to 56 us for the 64 sequences of 197, but 885 and 878 for 16384 keys).
+// does), an issuing warp per tile (the tiles fall into step: 1088 us).
 #include "attention_common.cuh"
 
 namespace {
@@ -188,12 +188,13 @@ __device__ __forceinline__ bool make_item(const Params &p, int block, int parts,
     return true;
 }
 
-template <int CH>
+template <int CH, bool kShort>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const Params p, int parts) {
     using Sh = Shape<CH>;
     constexpr int kStages = Sh::kStages, kBlock = Sh::kBlock;
+    constexpr int kTileUnroll = kShort ? 1 : 2;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Item s_items[kSlots];
     __shared__ alignas(16) uint4 s_stolen;
@@ -374,7 +375,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 return any;
             };
             int st = 0;
-            uint32_t ph = 0, blocks_done[2] = {0, 0}, tiles_q[2] = {0, 0}, tiles_o[2] = {0, 0};
+            uint32_t ph = 0, blocks_done = 0, tiles_q = 0, tiles_o = 0;  // phases, a bit per tile
             const auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
                 if (!failed && !warp_wait(bar, parity, p.status, code)) failed = true;
             };
@@ -390,7 +391,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             // scores of tile h for block j of an item
             const auto scores = [&](const Work &w, int h, int j, int stage) {
                 if (j >= w.n(h)) return;
-                if (j == 0) wait(&q_full[h], tiles_q[h]++ & 1, kWaitFull);
+                if (j == 0) {
+                    wait(&q_full[h], tiles_q >> h & 1, kWaitFull);
+                    tiles_q ^= 1u << h;
+                }
                 tc_fence_after();
                 const uint32_t idesc_s = idesc_bf16_f32(kRows, min((w.sees(h) - j * kKeys + 15) & ~15, kKeys));  // keys that are seen
                 if (!failed && elect_one()) {
@@ -436,13 +440,16 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     __syncwarp();
                 }
                 const uint32_t dv = ring_v + stage_v * (kBlock >> 4);
-#pragma unroll
+#pragma unroll kTileUnroll
                 for (int h = 0; h < 2; h++) {
                     const uint32_t t_s = tmem + h * kKeys, t_o = tmem + 256 + h * 128;
-                    const uint32_t parity = blocks_done[h] & 1;
+                    const uint32_t parity = blocks_done >> h & 1;
                     if (j + 1 < now.n(h) && dk == CH * 4) {
-                        blocks_done[h]++;
-                        if (j == 0) wait(&o_empty[h], (tiles_o[h]++ & 1) ^ 1, kWaitTmemEmpty);
+                        blocks_done ^= 1u << h;
+                        if (j == 0) {
+                            wait(&o_empty[h], tiles_o >> h & 1 ^ 1, kWaitTmemEmpty);
+                            tiles_o ^= 1u << h;
+                        }
                         wait(&p_half[h], parity, kWaitTmemEmpty);
                         tc_fence_after();
                         if (!failed && elect_one()) {
@@ -472,8 +479,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     }
                     if (j < now.n(h)) {
                         const int steps = (min(now.sees(h) - j * kKeys, kKeys) + 15) / 16;
-                        blocks_done[h]++;
-                        if (j == 0) wait(&o_empty[h], (tiles_o[h]++ & 1) ^ 1, kWaitTmemEmpty);
+                        blocks_done ^= 1u << h;
+                        if (j == 0) {
+                            wait(&o_empty[h], tiles_o >> h & 1 ^ 1, kWaitTmemEmpty);
+                            tiles_o ^= 1u << h;
+                        }
                         wait(&p_half[h], parity, kWaitTmemEmpty);
                         tc_fence_after();
                         if (!failed && elect_one()) {
@@ -665,7 +675,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         for (int c = 0; c < 32; c++) s[c0 + c] = seen & (1u << c) ? s[c0 + c] : -INFINITY;
                     }
                 }
-                if (j == 0) grow(largest<kKeys>(s));
+                if (!kShort && j == 0) grow(largest<kKeys>(s));
+                // (kShort: an item's first block has no maximum yet and goes around twice, the first time for that alone.)
                 // The first half's weights are taken relative to the maximum so far, while this block's is looked for: that is off the
                 // path between the products, and rarely are they to be done again.
                 uint64_t l_half;
@@ -673,10 +684,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 for (int pass = 0;; pass++) {
                     l_half = l;
                     const uint64_t b = base();
-                    weights(s, scale2, b, t_s, l_half);
+                    if (!kShort || j > 0 || pass > 0) weights(s, scale2, b, t_s, l_half);
                     const float top = largest<kKeys>(s);
-                    weights(s + 32, scale2, b, t_s + 16, l_half);
-                    const bool stays = (top - m) * p.scale_log2 <= kSlack || top == -INFINITY;
+                    if (!kShort || j > 0 || pass > 0) weights(s + 32, scale2, b, t_s + 16, l_half);
+                    const bool stays = (!kShort || j > 0) && ((top - m) * p.scale_log2 <= kSlack || top == -INFINITY);
                     if (pass == 1 || __all_sync(0xffffffffu, stays)) break;
                     grow(top);
                 }
@@ -715,12 +726,22 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     }
 }
 
+template <int CH, bool kShort>
+int launch_form(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV, int tiles,
+           int parts) {
+    SWC_CUDA(ctx, cudaFuncSetAttribute(attention_prompt_kernel<CH, kShort>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<CH>::kSmem));
+    attention_prompt_kernel<CH, kShort><<<(unsigned)tiles * p.units * parts, kThreads, Shape<CH>::kSmem, ctx->stream>>>(tmQ, tmK, tmV, p, parts);
+    return swc_check_launch(ctx, "attention_bf16");
+}
+
 template <int CH>
 int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV, int tiles,
            int parts) {
-    SWC_CUDA(ctx, cudaFuncSetAttribute(attention_prompt_kernel<CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<CH>::kSmem));
-    attention_prompt_kernel<CH><<<(unsigned)tiles * p.units * parts, kThreads, Shape<CH>::kSmem, ctx->stream>>>(tmQ, tmK, tmV, p, parts);
-    return swc_check_launch(ctx, "attention_bf16");
+    // The form with less code up to 1024 keys per sequence.  Short against long form, 16384 tokens in sequences of one length, 32
+    // heads, 8 key heads of 128, causal: 256 keys 111 / 115 us, 512 136 / 153, 1024 185 / 198, 2048 297 / 289; 16384 keys, 16 heads,
+    // 885 / 855.  Width 64, 16 heads, all keys: 64 sequences of 197 46 / 52 us, 32 of 1024 202 / 207.
+    return p.total_k / p.batch <= 1024 ? launch_form<CH, true>(ctx, p, tmQ, tmK, tmV, tiles, parts)
+                                       : launch_form<CH, false>(ctx, p, tmQ, tmK, tmV, tiles, parts);
 }
 
 }  // namespace

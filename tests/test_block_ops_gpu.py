@@ -346,6 +346,42 @@ def test_attention_prompts(be, lengths, hq, hkv, d, causal):
     attention_check(be, q, k, v, lengths, lengths, causal)
 
 
+# more than 1024 keys per sequence take another form of the kernel
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,hq,hkv,d", [([1025], 2, 2, 64), ([1024], 2, 2, 64), ([2100, 130], 8, 2, 128), ([1500], 7, 1, 72),
+                                              ([3000, 0, 520], 6, 3, 40), ([1, 2303, 1700], 4, 1, 96)])
+def test_attention_long_prompts(be, lengths, hq, hkv, d, causal):
+    rn = gen(sum(lengths) + d)
+    q, k, v = rn(sum(lengths), hq, d, dtype=BF16), rn(sum(lengths), hkv, d, dtype=BF16), rn(sum(lengths), hkv, d, dtype=BF16)
+    attention_check(be, q, k, v, lengths, lengths, causal)
+
+
+@pytest.mark.parametrize("flip", [False, True])
+def test_attention_long_prompts_scores_far_apart_and_not_finite(be, flip):
+    """As the two tests of that below, beyond 1024 keys."""
+    rn = gen(19)
+    new, n, d = 200, 2300, 64
+    q, k, v = rn(new, 2, d, dtype=BF16).abs(), rn(n, 2, d, dtype=BF16).abs(), rn(n, 2, d, dtype=BF16)
+    k = (k.float() * torch.linspace(-4, 40, n, device="cuda")[:, None, None]).to(BF16)
+    attention_check(be, q, k.flip(0).contiguous() if flip else k, v, [new], [n], False, scale=1.0)
+    clean = be.attention_bf16(q, k, v, offsets([new]), offsets([n]), causal=False)
+    q[5, 1, 3] = float("nan")
+    got = be.attention_bf16(q, k, v, offsets([new]), offsets([n]), causal=False)
+    assert got[5, 1].isnan().all() and torch.equal(got[:5], clean[:5]) and torch.equal(got[6:], clean[6:])
+
+
+@pytest.mark.parametrize("n", [300, 1500])
+def test_attention_keys_with_infinite_scores_below(be, n):
+    """Keys of score -infinity at the front, more than a block of them, weigh nothing."""
+    rn = gen(n)
+    new, d = 150, 64
+    q, k, v = rn(new, 2, d, dtype=BF16).abs() + 0.1, rn(n, 2, d, dtype=BF16), rn(n, 2, d, dtype=BF16)
+    k[:140, 0, :] = float("-inf")  # q > 0: every product is -infinity
+    got = be.attention_bf16(q, k, v, offsets([new]), offsets([n]), causal=False)
+    want, tol, _, _ = attention64(q[:, :1].contiguous(), k[140:, :1].contiguous(), v[140:, :1].contiguous(), new, n - 140, False, d ** -0.5)
+    check(got[:, :1], want, tol)
+
+
 @pytest.mark.parametrize("nq,nk,hq,hkv,d", [([1], [1], 1, 1, 8), ([1], [64], 4, 1, 128), ([1, 1, 1], [3000, 1, 700], 8, 2, 128), ([1] * 40, list(range(1, 2000, 50)), 8, 1, 64),
                                             ([4, 2], [1500, 2], 16, 2, 72), ([1], [5000], 64, 1, 128), ([1, 1], [900, 1300], 96, 1, 32),
                                             ([3, 0, 30, 1], [600, 5, 400, 0], 4, 4, 128), ([1], [9000], 128, 1, 16)])
