@@ -51,6 +51,20 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// A barrier of `nthreads` threads that also says whether `ok` held for all of them.
+__device__ __forceinline__ bool barrier_all(int id, int nthreads, bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)ok), "r"(id), "r"(nthreads)
+        : "memory");
+    return all != 0;
+}
+
 // items of a sequence for one unit of heads: pieces of its keys where its rows fit one tile, else its row tiles
 __device__ __forceinline__ int row_tiles(const Params &p, const Seq &s) { return (s.nq + p.tokens - 1) / p.tokens; }
 __device__ __forceinline__ int items_of(const Params &p, const Seq &s) {
@@ -231,7 +245,14 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
         const int k_row = kg * 16 + (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;   // K: (keys 0-7: d 0-7, 8-15), (keys 8-15: ..)
         const int v_row = kg * 16 + (lane & 15), v_piece = lane >> 4;                            // V: (keys 0-7, 8-15: d 0-7), (.. d 8-15)
         const int q_row = rg * 16 + (lane & 15), q_piece = lane >> 4;                            // Q: (rows 0-7, 8-15: d 0-7), (.. d 8-15)
-        for (; ok && next_item(item_full); items++) {
+        // The four warps of a row group leave together.  One whose wait has run out still comes to the item's first merge barrier,
+        // which tells the others, as they may have got what it waited for; no wait lies between that barrier and the next item.
+        for (;; items++) {
+            if (!next_item(item_full)) {
+                __syncwarp();
+                barrier_all(1 + rg, 128, ok);
+                break;
+            }
             // query fragments, rows g and g + 8 of this row group
             uint32_t qf[kD / 16][4];
             const uint32_t sq = smem_u32(q_tiles + (items & 1) * Sh::kQTile) + q_row * Sh::kQPitch + q_piece * 16;
@@ -322,7 +343,6 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 if (lane == 0) mbar_arrive(&empty[st]);
                 next();
             }
-            if (!ok) break;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -341,7 +361,13 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                         if (c2 == 0) *reinterpret_cast<float2 *>(r + kD) = make_float2(m[h], l[h]);
                     }
                 }
-                named_barrier(1 + rg, 128);
+                if (step == 2) {
+                    __syncwarp();
+                    ok = barrier_all(1 + rg, 128, ok);
+                    if (!ok) break;
+                } else {
+                    named_barrier(1 + rg, 128);
+                }
                 if (kg < step) {
                     const float *src = merge + (rg * 2 + kg) * 16 * kPitch;
 #pragma unroll
@@ -364,6 +390,7 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                 }
                 named_barrier(1 + rg, 128);
             }
+            if (!ok) break;
             if (kg == 0) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
