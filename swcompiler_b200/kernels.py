@@ -42,6 +42,7 @@ _FC_EPILOGUE = struct.Struct("@PifPii")
 _NORM_BLOCK = struct.Struct("@PiN" "iPPf4x" "PiNqf" "PiN" "PiN" "iPPf4x" "PiN")
 _ATTENTION = struct.Struct("@5P8N6i3PfiPN")
 _DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
+_INT_MAX = 2 ** 31 - 1  # ctypes drops what a C int cannot hold without a word
 
 
 class Backend:
@@ -128,6 +129,8 @@ class Backend:
         if dtype is None or t.ndim != 2 or t.get_device() != self._index:
             raise ValueError(f"{what}: expected an fp32 or bf16 matrix on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         rows, cols = t.shape
+        if cols > _INT_MAX:
+            raise ValueError(f"{what}: at most 2^31 - 1 columns, got {cols}")
         if t.is_contiguous():
             return t.data_ptr(), dtype, cols, rows, cols
         pitch, step = t.stride()
@@ -385,6 +388,8 @@ class Backend:
             pr, tr, ldr, rows, cols = self._matrix(what, residual)
             if rows != m or cols != n:
                 raise ValueError("fc_bf16_residual: residual and out are [m, n]")
+        if max(m, n, lda, ldw, ldr) > _INT_MAX:
+            raise ValueError("fc_bf16_residual: sizes and pitches are at most 2^31 - 1")
         if out is None:
             out = torch.empty(m, n, dtype=out_dtype, device=self.device)
             pc, tc, ldc = out.data_ptr(), _DTYPES[out_dtype], n
@@ -392,6 +397,8 @@ class Backend:
             pc, tc, ldc, rows, cols = self._matrix(what, out)
             if rows != m or cols != n:
                 raise ValueError("fc_bf16_residual: residual and out are [m, n]")
+            if ldc > _INT_MAX:
+                raise ValueError("fc_bf16_residual: sizes and pitches are at most 2^31 - 1")
         rc = self.lib.swcb200_fc_bf16_residual(self._ctx, m, n, k, pa, lda, pw, ldw,
                                                _FC_EPILOGUE.pack(self._vector(what, bias, n), act, scale, pr, tr, ldr), pc, tc, ldc)
         if rc:
