@@ -34,11 +34,11 @@ struct Seq {
 // nothing outside q, k, v, o is touched.
 __device__ __forceinline__ Seq load_seq(const Params &p, int b) {
     Seq s;
-    s.q0 = min(max(__ldg(p.q_off + b), 0), p.total_q);
-    s.nq = max(min(__ldg(p.q_off + b + 1), p.total_q), s.q0) - s.q0;  // (the lower bound first: no offset overflows)
-    s.k0 = min(max(__ldg(p.k_off + b), 0), p.total_k);
-    s.nk = max(min(__ldg(p.k_off + b + 1), p.total_k), s.k0) - s.k0;
-    if (p.k_lens) s.nk = min(max(__ldg(p.k_lens + b), 0), s.nk);
+    s.q0 = min(max(p.q_off[b], 0), p.total_q);
+    s.nq = max(min(p.q_off[b + 1], p.total_q), s.q0) - s.q0;  // (the lower bound first: no offset overflows)
+    s.k0 = min(max(p.k_off[b], 0), p.total_k);
+    s.nk = max(min(p.k_off[b + 1], p.total_k), s.k0) - s.k0;
+    if (p.k_lens) s.nk = min(max(p.k_lens[b], 0), s.nk);
     return s;
 }
 

@@ -72,6 +72,9 @@ static inline bool swc_aligned16(const void *p) { return (reinterpret_cast<uintp
 // Launch of a kernel that may start while the stream's previous kernel still runs: it sets itself up, then waits with
 // swc_after_previous() before it touches anything the previous kernel wrote.  A kernel that has called swc_let_next_start() in
 // all of its blocks lets such a successor take the SMs' free resources at once.
+// Such a kernel reads tensors with ordinary loads only: a non-coherent load (__ldg, ld.global.nc, a const __restrict__ parameter)
+// promises memory that nobody writes while the kernel runs, and the previous kernel, whose results these are, still ran when it
+// started.
 template <class... P, class... A>
 static inline cudaError_t swc_launch_early(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
                                            unsigned cluster, A... args) {

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
         failed = !__shfl_sync(0xffffffffu, ok, 0);
         tc_fence_after();
         if (!failed && p.splits == 1) {
-            const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
+            const float bias = p.bias && col < p.n ? p.bias[col] : 0.f;
             for (int c0 = half * 16; c0 < p.bn; c0 += 32) {
                 if (tm * p.bn + c0 >= p.m) break;
                 uint32_t r[16];
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kSplitThreads) fc_res_split_kernel(const __gri
         }
         cluster_sync();  // all partial sums have arrived
         if (warp >= 2) {
-            const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
+            const float bias = p.bias && col < p.n ? p.bias[col] : 0.f;
             // the CTA's tokens, half of them for each of the two warps of a quarter
             const int count = own > 2 ? own / 2 : half == 0 ? own : 0, first = count * half, slot = own * BM;
             const float *mine = slots + first * BM + row;
@@ -349,8 +349,8 @@ __device__ __noinline__ uint4 load_end(const __nv_bfloat16 *p, int count) {
 }
 
 template <int kTokens>
-__global__ void __launch_bounds__(kFewThreads, kTokens == 1 ? 4 : 1) fc_res_few_kernel(const __nv_bfloat16 *__restrict__ a, size_t lda,
-                                                                 const __nv_bfloat16 *__restrict__ w, size_t ldw, const FcrParams p) {
+__global__ void __launch_bounds__(kFewThreads, kTokens == 1 ? 4 : 1) fc_res_few_kernel(const __nv_bfloat16 *a, size_t lda,
+                                                                 const __nv_bfloat16 *w, size_t ldw, const FcrParams p) {
     constexpr int kFewRows = few_rows(kTokens), kV = kFewRows * kTokens;
     __shared__ float part[kFewThreads / 32][kV];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -368,12 +368,12 @@ __global__ void __launch_bounds__(kFewThreads, kTokens == 1 ? 4 : 1) fc_res_few_
 #pragma unroll
             for (int r = 0; r < kFewRows; r++) {
                 const __nv_bfloat16 *src = w + (size_t)min(n0 + r, p.n - 1) * ldw + k;
-                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(wv[r].x), "=r"(wv[r].y), "=r"(wv[r].z), "=r"(wv[r].w)
                              : "l"(src));
             }
 #pragma unroll
-            for (int t = 0; t < kTokens; t++) av[t] = __ldg(reinterpret_cast<const uint4 *>(a + (size_t)min(t, p.m - 1) * lda + k));
+            for (int t = 0; t < kTokens; t++) av[t] = *reinterpret_cast<const uint4 *>(a + (size_t)min(t, p.m - 1) * lda + k);
         } else {  // the end of the rows: nothing behind it is read
 #pragma unroll
             for (int r = 0; r < kFewRows; r++) wv[r] = load_end(w + (size_t)min(n0 + r, p.n - 1) * ldw + k, p.k - k);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kFewThreads, kTokens == 1 ? 4 : 1) fc_res_few_
         float v[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < kFewThreads / 32; i++) v[0] += part[i][threadIdx.x];
-        if (col < p.n) finish<1>(p, v, t, col, p.bias ? __ldg(p.bias + col) : 0.f);
+        if (col < p.n) finish<1>(p, v, t, col, p.bias ? p.bias[col] : 0.f);
     }
 }
 
@@ -549,7 +549,7 @@ fc_res_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             }
             tc_fence_after();
             const int col = tn * (2 * BM) + (int)rank * BM + quarter * 32 + lane;
-            const float bias = p.bias && col < p.n ? __ldg(p.bias + col) : 0.f;
+            const float bias = p.bias && col < p.n ? p.bias[col] : 0.f;
             for (int c0 = half * half_bn; c0 < (half + 1) * half_bn; c0 += 32) {
                 if (tm * p.bn + c0 >= p.m) break;
                 uint32_t r[32];

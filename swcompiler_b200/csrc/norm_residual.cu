@@ -120,7 +120,7 @@ __device__ __forceinline__ void store8(void *p, size_t i, bool is16, const float
 
 // the per-channel vectors: every row reads them, so they stay in L1
 __device__ __forceinline__ void vector8(const float *p, int i, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p + i)), b = __ldg(reinterpret_cast<const float4 *>(p + i) + 1);
+    const float4 a = *reinterpret_cast<const float4 *>(p + i), b = *reinterpret_cast<const float4 *>(p + i + 4);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
@@ -137,7 +137,7 @@ __device__ __forceinline__ void vector_chunks(const float *v, const RowParams &p
 #pragma unroll
             for (int e = 0; e < 8; e++) out[i * 8 + e] = x[e];
         } else {
-            out[i] = c < cols ? __ldg(v + c) : 0.f;
+            out[i] = c < cols ? v[c] : 0.f;
         }
     }
 }
@@ -232,8 +232,8 @@ norm_residual_kernel(const RowParams p) {
                 const int c = (i * p.tpr + tid) * kVec;
                 const __nv_bfloat16 *src = reinterpret_cast<const __nv_bfloat16 *>(p.gate) + base + c;
                 uint32_t v[4] = {0u, 0u, 0u, 0u};
-                if (kVec == 8 && c < cols) *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(src));
-                if (kVec == 1 && c < cols) v[0] = (uint32_t)__bfloat16_as_ushort(__ldg(src));
+                if (kVec == 8 && c < cols) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(src);
+                if (kVec == 1 && c < cols) v[0] = (uint32_t)__bfloat16_as_ushort(*src);
 #pragma unroll
                 for (int e = 0; e < kVec; e++) g[i * kVec + e] = __uint_as_float(e & 1 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16);
             }

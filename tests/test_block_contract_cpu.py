@@ -1,5 +1,8 @@
 """CPU: arguments that the transformer-block calls must not let through to the library."""
 import ctypes as C
+import glob
+import os
+import re
 
 import pytest
 import torch
@@ -9,6 +12,7 @@ from swcompiler_b200 import _lib as L
 from swcompiler_b200 import kernels as K
 
 BF16, F32 = torch.bfloat16, torch.float32
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "swcompiler_b200", "csrc")
 
 
 @pytest.fixture
@@ -54,3 +58,20 @@ def test_norm_residual_sizes_that_a_c_int_cannot_hold(be):
             be.norm_residual(meta(1, cols), pre=rms)
         with pytest.raises(ValueError):
             be.norm_residual(meta(2, cols))
+
+
+def test_kernels_that_start_early_use_ordinary_loads():
+    """A kernel that starts while its predecessor still writes must not read through non-coherent loads, which are for memory that
+    nobody writes while the kernel runs: neither by name nor by a const __restrict__ parameter, from which the compiler makes them."""
+    early = [f for f in glob.glob(os.path.join(CSRC, "*.cu")) if "swc_after_previous()" in open(f).read()]
+    assert len(early) >= 3
+    todo, seen = list(early), set()
+    while todo:
+        path = todo.pop()
+        if path in seen:
+            continue
+        seen.add(path)
+        text = re.sub(r"//[^\n]*|/\*.*?\*/", "", open(path).read(), flags=re.S)
+        todo += [os.path.join(CSRC, h) for h in re.findall(r'#include "(\w+\.cuh)"', text)]
+        found = re.findall(r"__ldg|__ldcs|\.global\.nc|ld_nc|__restrict__", text)
+        assert not found, (os.path.basename(path), found)

@@ -33,3 +33,44 @@ def test_attention_waits_that_run_out_end_the_call(hq, d):
         else:
             check(got, want, tol)
     assert 20_000 in ran_out and 4_000_000_000 not in ran_out
+
+
+@pytest.mark.parametrize("m", [1, 2, 24])
+def test_a_chain_reads_what_the_call_before_it_wrote(m):
+    """Layers of a gated block over the same few buffers, captured and replayed with new inputs: every call's operands (rows, gate,
+    bias, norm weights) were rewritten just before.  The bits are those of the calls one by one with a wait behind each."""
+    d, layers = 1024, 5
+    s = torch.cuda.Stream()
+    rn = gen(m)
+    with torch.cuda.stream(s):
+        be = swc.Backend(0, swc.TC_BF16, stream=s)
+        w = [[rn(d, d, dtype=BF16, s=d ** -0.5) for _ in range(4)] for _ in range(layers)]
+        x0, x = rn(m, d), torch.empty(m, d, device="cuda")
+        h, a, g, y = (torch.empty(m, d, dtype=BF16, device="cuda") for _ in range(4))
+        vector = torch.empty(1, d, device="cuda")
+        keep = [torch.empty(m, d, device="cuda") for _ in range(layers)]
+
+        def run(behind):
+            be.norm_residual(x0, pre=(swc.NORM_RMS, None, None, 1e-6), sum=x, y=h), behind()
+            for i, (w1, w2, w3, w4) in enumerate(w):
+                be.fc_bf16_residual(h, w1, out=a), behind()
+                be.fc_bf16_residual(h, w2, act=swc.ACT_SILU, out=g), behind()
+                be.fc_bf16_residual(h[:1], w3, act=swc.ACT_TANH, out=vector), behind()
+                be.norm_residual(a, gate=g, gate_rows=1, pre=(swc.NORM_LAYER, vector[0], vector[0], 1e-5), want_sum=False, y=y), behind()
+                be.fc_bf16_residual(y, w4, vector[0], residual=x, out=x), behind()
+                be.norm_residual(x, post=(swc.NORM_RMS, vector[0], None, 1e-6), pre=(swc.NORM_RMS, None, vector[0], 1e-6), sum=keep[i], y=h), behind()
+
+        run(lambda: None)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            run(lambda: None)
+        for step in range(12):
+            for _ in range(2):  # (the first one leaves other values in all of the buffers)
+                x0.copy_(rn(m, d))
+                graph.replay()
+            got = [t.clone() for t in keep + [h]]
+            run(s.synchronize)
+            assert all(torch.equal(p, q) for p, q in zip(got, keep + [h])), step
+        be.sync()
+    s.synchronize()
