@@ -81,9 +81,11 @@ int swcb200_set_precision(swcb200_ctx *ctx, int precision);
  * SWCB200_ERR_TIMEOUT; the context stays usable.  The limit is counted in SM clock cycles, 4e9 by
  * default (2 to 3 seconds).  The reference has no counterpart (its kernels cannot wait). */
 int swcb200_set_wait_limit(swcb200_ctx *ctx, long long cycles);
-/* The persistent tensor-core kernels (swcb200_fc_bf16*, swcb200_conv2d_bf16) launched through this context take at
- * most `sms` SMs (0 = all, the default).  They hold nearly all of an SM's shared memory, so a kernel of another
- * stream -- a collective that should run BESIDE a GEMM -- only finds room on SMs left free this way. */
+/* The tensor-core kernels (swcb200_fc_bf16*, swcb200_conv2d_bf16, swcb200_attention_bf16) launched through this context take
+ * at most `sms` SMs (0 = all, the default).  They hold much of an SM's shared memory, so a kernel of another
+ * stream -- a collective that should run BESIDE a GEMM -- only finds room on SMs left free this way.  (CTA pairs take two
+ * SMs at least.  Kernels that hold next to no shared memory take what there is: swcb200_fc_bf16_residual of one or two rows, and the
+ * join of swcb200_attention_bf16's parts.) */
 int swcb200_set_sm_limit(swcb200_ctx *ctx, int sms);
 /* Self-test of that path: launches one thread that waits, with the same bounded wait, on a barrier
  * nothing arrives at.  After the context's limit the kernel returns and swcb200_sync reports

@@ -13,7 +13,8 @@
 //     tile's softmax runs; it goes on across work items, so the first scores of the next item are there when one ends.
 //   * warp 13: TMA loads: query tiles when their last products have been issued, K and V blocks into a ring.
 //   * warp 14: work items.  The grid has one block per item; a resident CTA takes over blocks that have not started yet (cluster
-//     launch control), finds their sequence and hands the item to the other warps ahead of time.
+//     launch control), finds their sequence and hands the item to the other warps ahead of time.  Under an SM limit there is one
+//     CTA for each SM, and they take the blocks by stride.
 // Tensor memory: scores 2 x 128 columns, outputs 2 x 128 columns, all 512.  Head widths up to 64 use one 128-byte chunk per row,
 // up to 128 two; TMA fills the rest with zeros.
 // What bounds it: a block of a tile costs 1024 cycles of tensor pipe at width 128 (512 at 64) and 1024 of the exponential unit (16
@@ -188,10 +189,11 @@ __device__ __forceinline__ bool make_item(const Params &p, int block, int parts,
     return true;
 }
 
-template <int CH, bool kShort>
+// kStrided: for a grid of fewer CTAs than blocks.  (Compiled apart: a branch in the others cost them 1 %.)
+template <int CH, bool kShort, bool kStrided>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                        const __grid_constant__ CUtensorMap tmV, const Params p, int parts) {
+                        const __grid_constant__ CUtensorMap tmV, const Params p, int parts, int blocks) {
     using Sh = Shape<CH>;
     constexpr int kStages = Sh::kStages, kBlock = Sh::kBlock;
     constexpr int kTileUnroll = kShort ? 1 : 2;
@@ -284,7 +286,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             int block = blockIdx.x;
             uint32_t count = 0, asked = 0;
             while (!failed) {
-                if (lane == 0) {  // ask for the block after this one
+                if (lane == 0 && !kStrided) {  // ask for the block after this one
                     fence_proxy_async();
                     mbar_expect_tx(stolen, 16);
                     steal_block(&s_stolen, stolen);
@@ -299,6 +301,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                         mbar_arrive(&item_full[slot]);
                     }
                     __syncwarp();
+                }
+                if constexpr (kStrided) {
+                    if (blocks - block <= (int)gridDim.x) break;
+                    block += gridDim.x;
+                    continue;
                 }
                 if (!warp_wait(stolen, asked++ & 1, p.status, kWaitFull)) failed = true;
                 block = stolen_block(&s_stolen);
@@ -726,11 +733,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     }
 }
 
-template <int CH, bool kShort>
-int launch_form(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV, int tiles,
-           int parts) {
-    SWC_CUDA(ctx, cudaFuncSetAttribute(attention_prompt_kernel<CH, kShort>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<CH>::kSmem));
-    attention_prompt_kernel<CH, kShort><<<(unsigned)tiles * p.units * parts, kThreads, Shape<CH>::kSmem, ctx->stream>>>(tmQ, tmK, tmV, p, parts);
+template <int CH, bool kShort, bool kStrided = false>
+int launch_form(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV, int parts,
+                int blocks, int grid) {
+    const auto kernel = attention_prompt_kernel<CH, kShort, kStrided>;
+    SWC_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<CH>::kSmem));
+    kernel<<<(unsigned)grid, kThreads, Shape<CH>::kSmem, ctx->stream>>>(tmQ, tmK, tmV, p, parts, blocks);
     return swc_check_launch(ctx, "attention_bf16");
 }
 
@@ -740,8 +748,10 @@ int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const CUte
     // The form with less code up to 1024 keys per sequence.  Short against long form, 16384 tokens in sequences of one length, 32
     // heads, 8 key heads of 128, causal: 256 keys 111 / 115 us, 512 136 / 153, 1024 185 / 198, 2048 297 / 289; 16384 keys, 16 heads,
     // 885 / 855.  Width 64, 16 heads, all keys: 64 sequences of 197 46 / 52 us, 32 of 1024 202 / 207.
-    return p.total_k / p.batch <= 1024 ? launch_form<CH, true>(ctx, p, tmQ, tmK, tmV, tiles, parts)
-                                       : launch_form<CH, false>(ctx, p, tmQ, tmK, tmV, tiles, parts);
+    const int blocks = tiles * p.units * parts, sms = swc_tc_sms(ctx);
+    if (sms < ctx->sm_count && sms < blocks) return launch_form<CH, true, true>(ctx, p, tmQ, tmK, tmV, parts, blocks, sms);
+    return p.total_k / p.batch <= 1024 ? launch_form<CH, true>(ctx, p, tmQ, tmK, tmV, parts, blocks, blocks)
+                                       : launch_form<CH, false>(ctx, p, tmQ, tmK, tmV, parts, blocks, blocks);
 }
 
 }  // namespace

@@ -562,7 +562,9 @@ int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmK, const CUte
     const size_t smem = Shape<CH, RG>::kSmem;
     SWC_CUDA(ctx, cudaFuncSetAttribute(attention_token_kernel<CH, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const long long work = (long long)max_items * p.units;
-    const long long slots = (long long)ctx->sm_count * Shape<CH, RG>::kCtas;
+    // (under a limit one CTA for each SM: two would not share one, but take an SM each)
+    const int sms = swc_tc_sms(ctx);
+    const long long slots = sms < ctx->sm_count ? sms : (long long)sms * Shape<CH, RG>::kCtas;
     const unsigned grid = (unsigned)(work < slots ? work : slots);
     SWC_CUDA(ctx, swc_launch_early(attention_token_kernel<CH, RG>, grid, RG * 128 + 64, smem, ctx->stream, 1, tmK, tmV, p));
     return swc_check_launch(ctx, "attention_bf16");

@@ -597,7 +597,9 @@ struct Choice {
 // token; the join over 2 / 4 / 8 CTAs 0.8 / 2 / 3.5.  Forms compared in one run, (m, n) = (777, 1000): chosen 128 tokens over 2
 // CTAs 14.7 us; 4 CTAs (two waves) 21.6; undivided 19.9; 256 tokens over 4 18.1; pairs 26.1.  (64, 4096): 64 over 4 11.1; over 8
 // 12.4; undivided 17.7.
-Choice choose(int m, int n, int kblocks, int sms) {
+// limited: no more than `sms` CTAs at all, as each holds an SM of its own.  Only the pairs walk over tiles, so a split form is open
+// to calls of one wave; a limit of one SM gets a pair all the same.
+Choice choose(int m, int n, int kblocks, int sms, bool limited) {
     Choice best = {true, BN_MAX, 1};
     const auto up = [](long long a, long long b) { return (a + b - 1) / b; };
     double least = sms < 2 ? 1e30 : (double)up(up(n, 2 * BM) * up(m, BN_MAX), sms / 2) * kblocks * 0.30 + 6.5;
@@ -606,7 +608,9 @@ Choice choose(int m, int n, int kblocks, int sms) {
         for (int j = 0; j < 4; j++) {
             const int bn = 16 << i, s = 1 << j;
             if ((j > 0 && s * 2 > kblocks) || (i > 0 && bn >= 2 * m)) continue;
-            const double t = (double)up(up(n, BM) * up(m, bn) * s, sms) * ((double)up(kblocks, s) * step[i] + 6.5 + 0.016 * bn + join[j]);
+            const long long waves = up(up(n, BM) * up(m, bn) * s, sms);
+            if (limited && waves > 1) continue;
+            const double t = (double)waves * ((double)up(kblocks, s) * step[i] + 6.5 + 0.016 * bn + join[j]);
             if (t < least) least = t, best = {false, bn, s};
         }
     return best;
@@ -658,7 +662,7 @@ SWC_EXPORT int swcb200_fc_bf16_residual(swcb200_ctx *ctx, int m, int n, int k, c
         return swc_check_launch(ctx, "fc_bf16_residual");
     }
     const int kblocks = (k + BK - 1) / BK;
-    const Choice best = choose(m, n, kblocks, sms);
+    const Choice best = choose(m, n, kblocks, sms, sms < ctx->sm_count);
     p.bn = best.bn;
     p.splits = best.splits;
     p.tiles_m = (m + p.bn - 1) / p.bn;
@@ -670,7 +674,7 @@ SWC_EXPORT int swcb200_fc_bf16_residual(swcb200_ctx *ctx, int m, int n, int k, c
         if (!rc) rc = tmap_rows(ctx, a_bf16, m, k, lda, p.bn / 2, &tmA);
         if (rc) return rc;
         SWC_CUDA(ctx, cudaFuncSetAttribute(fc_res_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem));
-        const long long tiles = (long long)p.tiles_n * p.tiles_m, pairs = sms / 2;
+        const long long tiles = (long long)p.tiles_n * p.tiles_m, pairs = sms > 1 ? sms / 2 : 1;
         SWC_CUDA(ctx, swc_launch_early(fc_res_pair_kernel, 2u * (unsigned)(tiles < pairs ? tiles : pairs), kPairThreads, kPairSmem,
                                        ctx->stream, 1, tmW, tmA, p));
         return swc_check_launch(ctx, "fc_bf16_residual");

@@ -95,7 +95,7 @@ class Backend:
         self._call("set_wait_limit", C.c_longlong(cycles))
 
     def set_sm_limit(self, sms: int):
-        """The persistent tensor-core kernels of this context take at most `sms` SMs (0 = all): leaves room for a
+        """The tensor-core kernels of this context take at most `sms` SMs (0 = all): leaves room for a
         collective of another stream to run beside them."""
         self._call("set_sm_limit", C.c_int(sms))
 

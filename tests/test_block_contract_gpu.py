@@ -4,7 +4,7 @@ import torch
 
 import swcompiler_b200 as swc
 from swcompiler_b200 import _lib as L
-from test_block_ops_gpu import attention64, check, gen, offsets
+from test_block_ops_gpu import attention64, be, check, gen, offsets  # noqa: F401 (be: a fixture)
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -74,3 +74,57 @@ def test_a_chain_reads_what_the_call_before_it_wrote(m):
             assert all(torch.equal(p, q) for p, q in zip(got, keep + [h])), step
         be.sync()
     s.synchronize()
+
+
+def least_ms(be, call, times=6):
+    call()
+    best = float("inf")
+    for _ in range(times):
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        e[0].record()
+        call()
+        e[1].record()
+        e[1].synchronize()
+        best = min(best, e[0].elapsed_time(e[1]))
+    return best
+
+
+@pytest.mark.parametrize("what", ["split", "pairs", "tokens", "many rows", "prompts", "long prompt", "chunk"])
+def test_an_sm_limit_holds(be, what):
+    """With eight SMs of all of them a call takes many times as long (a quarter of the SMs' ratio is asked for), and its results are
+    right under any limit."""
+    rn = gen(len(what))
+    if what in ("split", "pairs"):
+        m, n, k = (64, 8192, 4096) if what == "split" else (4096, 4096, 2048)
+        a, wp, out = rn(m, k, dtype=BF16), rn(n, k, dtype=BF16, s=k ** -0.5), torch.empty(m, n, device="cuda")
+        want = a.double() @ wp.double().t()
+        tol = k / 16 * 2 ** -22 * (a.double().abs() @ wp.double().abs().t())
+
+        def call():
+            be.fc_bf16_residual(a, wp, out=out)
+    else:
+        nq, nk, hq, hkv, d = {"tokens": ([1] * 64, [2000] * 64, 8, 8, 128), "many rows": ([2] * 16, [3000] * 16, 64, 2, 64),
+                              "prompts": ([200] * 64, [200] * 64, 16, 8, 64), "long prompt": ([4000], [4000], 16, 2, 128),
+                              "chunk": ([70], [40000], 8, 2, 128)}[what]
+        q, k, v = rn(sum(nq), hq, d, dtype=BF16), rn(sum(nk), hkv, d, dtype=BF16), rn(sum(nk), hkv, d, dtype=BF16)
+        off_q, off_k, out = offsets(nq), offsets(nk), torch.empty(sum(nq), hq, d, dtype=BF16, device="cuda")
+        parts = [attention64(q[i * nq[0]:(i + 1) * nq[0]], k[i * nk[0]:(i + 1) * nk[0]], v[i * nk[0]:(i + 1) * nk[0]], nq[0], nk[0], True, d ** -0.5)[:2]
+                 for i in range(len(nq))]
+        want, tol = (torch.cat(t) for t in zip(*parts))
+
+        def call():
+            be.attention_bf16(q, k, v, off_q, off_k, out=out)
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    try:
+        free = least_ms(be, call)
+        for limit in (1, 8, 21, sms + 1):
+            be.set_sm_limit(limit)
+            out.fill_(float("nan"))
+            t = least_ms(be, call)
+            check(out, want, tol)
+            if limit == 8:
+                assert t > free * sms / 8 / 4, (t, free)
+    finally:
+        be.set_sm_limit(0)
+    be.sync()
