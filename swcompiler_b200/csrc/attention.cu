@@ -69,6 +69,7 @@ int make_plan(swcb200_ctx *ctx, const swcb200_attention *a, Plan &pl) {
     return SWCB200_OK;
 }
 
+// the fields that the workspace's size follows from
 int check(swcb200_ctx *ctx, const swcb200_attention *a) {
     SWC_REQUIRE(ctx, a != nullptr, SWCB200_ERR_BAD_ARG, "attention_bf16: null description");
     SWC_REQUIRE(ctx, a->batch >= 0 && a->total_q >= 0 && a->total_k >= 0 && a->heads_q >= 1 && a->heads_kv >= 1 && a->head_dim >= 1,
@@ -79,7 +80,6 @@ int check(swcb200_ctx *ctx, const swcb200_attention *a) {
                 "attention_bf16: %d query heads are no multiple of %d key heads", a->heads_q, a->heads_kv);
     SWC_REQUIRE(ctx, a->head_dim % 8 == 0 && a->head_dim <= 128, SWCB200_ERR_UNSUPPORTED,
                 "attention_bf16: head width %d (multiples of 8 up to 128)", a->head_dim);
-    SWC_REQUIRE(ctx, a->scale > 0.f && a->scale <= 3.4e38f, SWCB200_ERR_BAD_ARG, "attention_bf16: the scale must be positive and finite");
     return SWCB200_OK;
 }
 
@@ -132,7 +132,9 @@ SWC_EXPORT int swcb200_attention_workspace(swcb200_ctx *ctx, const swcb200_atten
 SWC_EXPORT int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention *a) {
     SWC_CTX(ctx);
     int rc = check(ctx, a);
-    if (rc || a->batch == 0 || a->total_q == 0) return rc;
+    if (rc) return rc;
+    SWC_REQUIRE(ctx, a->scale > 0.f && a->scale <= 3.4e38f, SWCB200_ERR_BAD_ARG, "attention_bf16: the scale must be positive and finite");
+    if (a->batch == 0 || a->total_q == 0) return SWCB200_OK;
     SWC_REQUIRE(ctx, a->q && a->o && (a->total_k == 0 || (a->k && a->v)) && a->q_offsets && a->k_offsets, SWCB200_ERR_BAD_ARG,
                 "attention_bf16: null tensor");
     // (with no keys at all every row is empty: q stands in for the tensors that nothing is read from)

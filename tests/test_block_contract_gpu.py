@@ -1,9 +1,12 @@
 """GPU: what the transformer-block calls promise beside their results: bounded waits, limits, order on a stream."""
+import ctypes as C
+
 import pytest
 import torch
 
 import swcompiler_b200 as swc
 from swcompiler_b200 import _lib as L
+from swcompiler_b200 import kernels as K
 from test_block_ops_gpu import attention64, be, check, gen, offsets  # noqa: F401 (be: a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -128,3 +131,20 @@ def test_an_sm_limit_holds(be, what):
     finally:
         be.set_sm_limit(0)
     be.sync()
+
+
+def test_attention_workspace_reads_no_more_than_it_says(be):
+    """Batch, totals, heads and width, in a description that is zero otherwise: the bytes of the whole description."""
+    fields = [0] * 26
+    fields[13:19] = 1, 1, 60000, 32, 8, 128
+    need, whole = C.c_size_t(), C.c_size_t()
+    assert be.lib.swcb200_attention_workspace(be._ctx, K._ATTENTION.pack(*fields), C.byref(need)) == L.OK and need.value > 0
+    fields[22] = 0.1
+    assert be.lib.swcb200_attention_workspace(be._ctx, K._ATTENTION.pack(*fields), C.byref(whole)) == L.OK and whole.value == need.value
+    q, k = torch.zeros(1, 32, 128, dtype=BF16, device="cuda"), torch.zeros(600, 8, 128, dtype=BF16, device="cuda")
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(swc.SwcError) as e:
+            be.attention_bf16(q, k, k, offsets([1]), offsets([600]), scale=scale)
+        assert e.value.status == L.ERR_BAD_ARG
+    with pytest.raises(swc.SwcError):
+        be.attention_bf16(q[:0], k, k, offsets([0]), offsets([600]), scale=0.0)  # empty calls, too
