@@ -311,9 +311,10 @@ attention_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
                                 o[i][2 * h + 1] *= factor;
                             }
                         }
-                        const float base = m[h] == -INFINITY ? 0.f : m[h] * p.scale_log2;
+                        // (the difference first: x * scale - m * scale is off by the rounding of a product that has no bound)
+                        const float base = m[h] == -INFINITY ? 0.f : m[h];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) x[i] = exp2_fast(fmaf(x[i], p.scale_log2, -base));
+                        for (int i = 0; i < 4; i++) x[i] = exp2_fast((x[i] - base) * p.scale_log2);
                         l[h] += (x[0] + x[1]) + (x[2] + x[3]);
                         w[h] = pack_bf16(x[0], x[1]);
                         w[h + 2] = pack_bf16(x[2], x[3]);

@@ -148,3 +148,27 @@ def test_attention_workspace_reads_no_more_than_it_says(be):
         assert e.value.status == L.ERR_BAD_ARG
     with pytest.raises(swc.SwcError):
         be.attention_bf16(q[:0], k, k, offsets([0]), offsets([600]), scale=0.0)  # empty calls, too
+
+
+@pytest.mark.parametrize("new,n", [(1, 900), (30, 700), (200, 900), (200, 2300), (70, 6000)])
+@pytest.mark.parametrize("size", [3e3, 3e4, 1e6, 1e12])
+def test_attention_scores_far_beyond_the_exponential(be, new, n, size):
+    """Scores of 1e7 up to 1e25: a row is the value of its largest score.  All terms of a score are positive, so it is known to
+    (d / 16 + 1) * 2^-22 of itself; rows whose two largest scores are nearer than four times that are left out.  The one weight left is
+    rounded to bf16."""
+    d, h = 64, 2
+    rn = gen(new + n)
+    q, k, v = (rn(new, h, d).abs() * size).to(BF16), (rn(n, h, d).abs() * size).to(BF16), rn(n, h, d, dtype=BF16)
+    slope = torch.linspace(0.5, 2, n, device="cuda")[:, None, None]
+    for keys in (k, (k.float() * slope).to(BF16), (k.float() * slope.flip(0)).to(BF16)):
+        lse = torch.empty(new, h, device="cuda")
+        got = be.attention_bf16(q, keys, v, offsets([new]), offsets([n]), causal=False, lse=lse)
+        s = d ** -0.5 * q.double().transpose(0, 1) @ keys.double().permute(1, 2, 0)
+        first, second = s.topk(2, 2).values.unbind(2)
+        known = (d / 16 + 1) * 2 ** -22
+        clear = (first - second > 4 * known * first).t()
+        assert clear.float().mean() > 0.9
+        want = torch.stack([v[s[i].argmax(1), i] for i in range(h)], 1).double()
+        check(got[clear], want[clear], 2 ** -8 * want[clear].abs())
+        assert ((lse.double() - first.t()).abs() <= (known + 2 ** -21) * first.t()).all()
+    be.sync()
