@@ -326,7 +326,7 @@ typedef struct swcb200_attention {
     int batch, total_q, total_k, heads_q, heads_kv, head_dim;
     const int *q_offsets, *k_offsets; /* [batch + 1] */
     const int *k_lens;                /* [batch] or NULL */
-    float scale;                      /* > 0 */
+    float scale;                      /* > 0, at most 2e38 */
     int causal;
     void *workspace; /* 16-byte aligned; may be NULL where swcb200_attention_workspace says 0 */
     size_t workspace_bytes;

@@ -1,4 +1,6 @@
 // Attention entry points: argument checks, and which kernel takes a call.
+#include <float.h>
+
 #include "attention_common.cuh"
 
 using namespace attn;
@@ -133,7 +135,8 @@ SWC_EXPORT int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention 
     SWC_CTX(ctx);
     int rc = check(ctx, a);
     if (rc) return rc;
-    SWC_REQUIRE(ctx, a->scale > 0.f && a->scale <= 3.4e38f, SWCB200_ERR_BAD_ARG, "attention_bf16: the scale must be positive and finite");
+    const float scale_log2 = a->scale * 1.4426950408889634f;  // finite, too
+    SWC_REQUIRE(ctx, a->scale > 0.f && scale_log2 <= FLT_MAX, SWCB200_ERR_BAD_ARG, "attention_bf16: the scale must be positive and at most 2e38");
     if (a->batch == 0 || a->total_q == 0) return SWCB200_OK;
     SWC_REQUIRE(ctx, a->q && a->o && (a->total_k == 0 || (a->k && a->v)) && a->q_offsets && a->k_offsets, SWCB200_ERR_BAD_ARG,
                 "attention_bf16: null tensor");
@@ -158,7 +161,7 @@ SWC_EXPORT int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention 
     p.batch = a->batch, p.total_q = a->total_q, p.total_k = a->total_k;
     p.heads_q = a->heads_q, p.group = a->heads_q / a->heads_kv, p.d = a->head_dim;
     p.pack = pl.pack, p.pack_inv = (65536u + pl.pack - 1) / pl.pack, p.units = pl.units, p.tokens = pl.tokens;
-    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.scale_log2 = scale_log2;
     p.causal = a->causal != 0;
     p.part = pl.part, p.max_items = pl.max_items;
     p.part_o = (float *)a->workspace;

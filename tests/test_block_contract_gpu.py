@@ -172,3 +172,19 @@ def test_attention_scores_far_beyond_the_exponential(be, new, n, size):
         check(got[clear], want[clear], 2 ** -8 * want[clear].abs())
         assert ((lse.double() - first.t()).abs() <= (known + 2 ** -21) * first.t()).all()
     be.sync()
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_attention_largest_and_smallest_scales(be, new):
+    """The softmax runs on powers of two: a scale that is finite, but not times log2(e), is refused; smaller ones give no NaN."""
+    rn = gen(new)
+    q, k, v = rn(new, 2, 64, dtype=BF16), rn(300, 2, 64, dtype=BF16), rn(300, 2, 64, dtype=BF16)
+    for scale in (2.4e38, 3.3e38):
+        with pytest.raises(swc.SwcError) as e:
+            be.attention_bf16(q * 0, k, v, offsets([new]), offsets([300]), scale=scale)
+        assert e.value.status == L.ERR_BAD_ARG
+    uniform = v.double().mean(0, keepdim=True).expand(new, 2, 64)
+    # equal weights: 300 of them, rounded to bf16 (1 is a bf16), and 300 additions of the products
+    tol = 300 * 2 ** -24 * v.double().abs().mean(0)
+    check(be.attention_bf16(q * 0, k, v, offsets([new]), offsets([300]), scale=2e38, causal=False), uniform, tol)
+    check(be.attention_bf16(q, k, v, offsets([new]), offsets([300]), scale=1e-30, causal=False), uniform, tol)
