@@ -148,6 +148,14 @@ class Backend:
             raise ValueError(f"{what}: expected a contiguous fp32 vector of {n} elements on {self.device}")
         return t.data_ptr()
 
+    def _result(self, what, rows, cols, dtype):
+        """A new fp32 or bf16 matrix, its address and its dtype."""
+        code = _DTYPES.get(dtype)
+        if code is None:
+            raise ValueError(f"{what}: results are fp32 or bf16, not {dtype}")
+        t = torch.empty(rows, cols, dtype=dtype, device=self.device)
+        return t, t.data_ptr(), code
+
     def _new(self, shape, dtype=torch.float32):
         return torch.empty(tuple(int(s) for s in shape), dtype=dtype, device=self.device)
 
@@ -391,8 +399,7 @@ class Backend:
         if max(m, n, lda, ldw, ldr) > _INT_MAX:
             raise ValueError("fc_bf16_residual: sizes and pitches are at most 2^31 - 1")
         if out is None:
-            out = torch.empty(m, n, dtype=out_dtype, device=self.device)
-            pc, tc, ldc = out.data_ptr(), _DTYPES[out_dtype], n
+            (out, pc, tc), ldc = self._result(what, m, n, out_dtype), n
         else:
             pc, tc, ldc, rows, cols = self._matrix(what, out)
             if rows != m or cols != n:
@@ -436,8 +443,7 @@ class Backend:
         if sum is None:
             if want_sum:
                 sum_dtype = sum_dtype or (x if residual is None else residual).dtype
-                sum = torch.empty(rows, cols, dtype=sum_dtype, device=self.device)
-                p_sum, t_sum, ld_sum = sum.data_ptr(), _DTYPES[sum_dtype], cols
+                (sum, p_sum, t_sum), ld_sum = self._result(what, rows, cols, sum_dtype), cols
         else:
             p_sum, t_sum, ld_sum, r, c = self._matrix(what, sum)
             if r != rows or c != cols:
@@ -447,8 +453,7 @@ class Backend:
             if r != rows or c != cols:
                 raise ValueError("norm_residual: tensors of different shapes")
         elif pre is not None:
-            y = torch.empty(rows, cols, dtype=y_dtype, device=self.device)
-            p_y, t_y, ld_y = y.data_ptr(), _DTYPES[y_dtype], cols
+            (y, p_y, t_y), ld_y = self._result(what, rows, cols, y_dtype), cols
         rc = self.lib.swcb200_norm_residual(
             self._ctx, rows, cols,
             _NORM_BLOCK.pack(px, tx, ldx, k_post, w_post, b_post, e_post, p_gate, t_gate, ld_gate, gate_rows, scale, p_res, t_res,

@@ -75,3 +75,12 @@ def test_kernels_that_start_early_use_ordinary_loads():
         todo += [os.path.join(CSRC, h) for h in re.findall(r'#include "(\w+\.cuh)"', text)]
         found = re.findall(r"__ldg|__ldcs|\.global\.nc|ld_nc|__restrict__", text)
         assert not found, (os.path.basename(path), found)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.int32])
+def test_results_of_other_types_are_refused(be, dtype):
+    x, rms = meta(4, 64), (swc.NORM_RMS, None, None, 1e-6)
+    for call in (lambda: be.fc_bf16_residual(x, meta(24, 64), out_dtype=dtype), lambda: be.norm_residual(x, pre=rms, sum_dtype=dtype),
+                 lambda: be.norm_residual(x, pre=rms, y_dtype=dtype), lambda: be.norm_residual(x, pre=rms, want_sum=False, y_dtype=dtype)):
+        with pytest.raises(ValueError):
+            call()
