@@ -7,7 +7,7 @@ import torch
 import swcompiler_b200 as swc
 from swcompiler_b200 import _lib as L
 from swcompiler_b200 import kernels as K
-from test_block_ops_gpu import attention64, be, check, gen, offsets  # noqa: F401 (be: a fixture)
+from test_block_ops_gpu import attention64, be, check, fc_check, gen, offsets  # noqa: F401 (be: a fixture)
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -188,3 +188,14 @@ def test_attention_largest_and_smallest_scales(be, new):
     tol = 300 * 2 ** -24 * v.double().abs().mean(0)
     check(be.attention_bf16(q * 0, k, v, offsets([new]), offsets([300]), scale=2e38, causal=False), uniform, tol)
     check(be.attention_bf16(q, k, v, offsets([new]), offsets([300]), scale=1e-30, causal=False), uniform, tol)
+
+
+@pytest.mark.parametrize("m,n,k", [(1900, 6500, 4104), (700, 4700, 5600)])
+def test_fc_bf16_residual_tiles_in_bands(be, m, n, k):
+    """Weights of more than 48 MiB in tiles of 256 whose number is no multiple of 8: tiles are taken in bands, the last one narrower.
+    Every tile is written, once (in place, a second time would add its product again)."""
+    rn = gen(n)
+    a, wp, bias, r = rn(m, k, dtype=BF16), rn(n, k, dtype=BF16, s=k ** -0.5), rn(n), rn(m, n)
+    out = r.clone()
+    be.fc_bf16_residual(a, wp, bias, residual=out, out=out)
+    fc_check(out, a, wp, bias, "NONE", r, 1.0)
