@@ -549,12 +549,11 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const Para
     if (lane == 0 && p.lse) p.lse[(size_t)token * p.heads_q + head] = l == 0.f ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
 }
 
-template <bool kItems> int join(swcb200_ctx *ctx, const Params &p, int rows, int parts, bool many) {
+template <bool kItems, int kWarps> int join(swcb200_ctx *ctx, const Params &p, int rows, int parts) {
+    constexpr int kRowsPerCta = kJoinThreads / 32 / kWarps;
     const long long all = (long long)p.total_q * p.heads_q;
-    if (many)
-        SWC_CUDA(ctx, swc_launch_early(attention_join_kernel<kItems, 8>, (unsigned)all, kJoinThreads, 0, ctx->stream, 1, p, rows, parts));
-    else
-        SWC_CUDA(ctx, swc_launch_early(attention_join_kernel<kItems, 1>, (unsigned)((all + 7) / 8), kJoinThreads, 0, ctx->stream, 1, p, rows, parts));
+    SWC_CUDA(ctx, swc_launch_early(attention_join_kernel<kItems, kWarps>, (unsigned)((all + kRowsPerCta - 1) / kRowsPerCta), kJoinThreads, 0,
+                                   ctx->stream, 1, p, rows, parts));
     return swc_check_launch(ctx, "attention_bf16");
 }
 
@@ -580,7 +579,7 @@ int swc_attention_token(swcb200_ctx *ctx, Params &p, const CUtensorMap &tmK, con
     else
         rc = rows == 16 ? launch<1, 1>(ctx, p, tmK, tmV, max_items) : rows == 32 ? launch<1, 2>(ctx, p, tmK, tmV, max_items) : launch<1, 4>(ctx, p, tmK, tmV, max_items);
     if (rc || p.part >= p.total_k) return rc;  // no sequence has more than one part
-    return join<true>(ctx, p, rows, 0, p.total_k / p.batch > 16ll * p.part);
+    return p.total_k / p.batch > 16ll * p.part ? join<true, 8>(ctx, p, rows, 0) : join<true, 1>(ctx, p, rows, 0);
 }
 
-int swc_attention_join_parts(swcb200_ctx *ctx, Params &p, int parts) { return join<false>(ctx, p, 0, parts, false); }
+int swc_attention_join_parts(swcb200_ctx *ctx, Params &p, int parts) { return join<false, 1>(ctx, p, 0, parts); }

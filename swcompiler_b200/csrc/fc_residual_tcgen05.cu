@@ -55,10 +55,6 @@ __device__ __forceinline__ float activate(float v) {
     return v;
 }
 
-__device__ __forceinline__ float load_elem(const void *p, bool is16, size_t i) {
-    return is16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]) : reinterpret_cast<const float *>(p)[i];
-}
-
 // kTok tokens of one output column: acc[j] belongs to token t0 + j
 template <int kAct, int kTok>
 __device__ __forceinline__ void finish_act(const FcrParams &p, const float (&acc)[kTok], int t0, int tokens, int col, float bias) {

@@ -280,9 +280,12 @@ norm_residual_kernel(const RowParams p) {
 
 template <int kVec, bool kCta, int kX, int kR> cudaError_t launch_types(int n, unsigned grid, int threads, cudaStream_t s, const RowParams &p) {
     constexpr int k = kVec == 8 ? 1 : 8;  // chunks of one element come in eights
-    const auto kernel = n <= k       ? norm_residual_kernel<kVec, k, kCta, kX, kR>
-                        : n <= 2 * k ? norm_residual_kernel<kVec, 2 * k, kCta, kX, kR>
-                                     : norm_residual_kernel<kVec, 4 * k, kCta, kX, kR>;
+    auto kernel = norm_residual_kernel<kVec, k, kCta, kX, kR>;
+    // (rows inside a warp have no more than two chunks of 8, or eight of one element, a thread)
+    if constexpr (kCta || kVec == 8)
+        if (n > k) kernel = norm_residual_kernel<kVec, 2 * k, kCta, kX, kR>;
+    if constexpr (kCta)
+        if (n > 2 * k) kernel = norm_residual_kernel<kVec, 4 * k, kCta, kX, kR>;
     return swc_launch_early(kernel, grid, (unsigned)threads, 0, s, 1, p);
 }
 template <bool kCta> cudaError_t launch(bool vec, int n, unsigned grid, int threads, cudaStream_t s, const RowParams &p) {
