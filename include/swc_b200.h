@@ -314,10 +314,10 @@ int swcb200_norm_residual(swcb200_ctx *ctx, size_t rows, int cols, const swcb200
  * within a sequence a value row that is not finite also reaches rows that the causal mask keeps
  * from it.  Scores, softmax and sums are fp32 (the weights are rounded to bf16 for the second
  * product).  Offsets are clamped to the tensors, which have at most 2^30 rows.  Alignment (TMA):
- * bases on 16 bytes, strides multiples of 8.  o may not overlap q, k or v (compared from first to
- * last element), and no other tensor of the call or the workspace may overlap what it writes.  The
- * workspace belongs to the call until it has finished on the stream: calls in flight together (two
- * captured graphs, too) need one each. */
+ * bases on 16 bytes, strides multiples of 8.  o may not overlap itself (one stride steps over all that
+ * the other one reaches) nor q, k or v (compared from first to last element), and no other tensor of the
+ * call or the workspace may overlap what it writes.  The workspace belongs to the
+ * call until it has finished on the stream: calls in flight together (two captured graphs, too) need one each. */
 typedef struct swcb200_attention {
     const void *q, *k, *v;
     void *o;

@@ -146,6 +146,9 @@ SWC_EXPORT int swcb200_attention_bf16(swcb200_ctx *ctx, const swcb200_attention 
     const Rows v = a->total_k ? Rows{a->v, a->v_row, a->v_head, a->total_k, a->heads_kv, "v"} : q;
     for (const Rows *t : {&q, &k, &v, &o})
         if ((rc = check_rows(ctx, *t, a->head_dim))) return rc;
+    // (several CTAs write o: one of its strides steps over all that the other one reaches)
+    SWC_REQUIRE(ctx, o.rows == 1 || o.heads == 1 || o.row >= (size_t)(o.heads - 1) * o.head + a->head_dim ||
+                o.head >= (size_t)(o.rows - 1) * o.row + a->head_dim, SWCB200_ERR_BAD_SHAPE, "attention_bf16: rows and heads of o overlap");
     for (const Rows *t : {&q, &k, &v})
         SWC_REQUIRE(ctx, !ranges_meet(*t, o, a->head_dim), SWCB200_ERR_BAD_ARG, "attention_bf16: o overlaps %s", t->name);
     Plan pl;

@@ -199,3 +199,19 @@ def test_fc_bf16_residual_tiles_in_bands(be, m, n, k):
     out = r.clone()
     be.fc_bf16_residual(a, wp, bias, residual=out, out=out)
     fc_check(out, a, wp, bias, "NONE", r, 1.0)
+
+
+@pytest.mark.parametrize("new", [2, 90])
+def test_attention_outputs_that_overlap_themselves_are_refused(be, new):
+    rn = gen(new)
+    q, k, v = rn(new, 4, 32, dtype=BF16), rn(200, 2, 32, dtype=BF16), rn(200, 2, 32, dtype=BF16)
+    room = torch.zeros(new * 4 * 64, dtype=BF16, device="cuda")
+    want = be.attention_bf16(q, k, v, offsets([new]), offsets([200]))
+    for strides in ((32, 32, 1), (96, 32, 1), (32, 32 * new - 8, 1), (40, 40, 1)):
+        with pytest.raises(swc.SwcError) as e:
+            be.attention_bf16(q, k, v, offsets([new]), offsets([200]), out=room.as_strided((new, 4, 32), strides))
+        assert e.value.status == L.ERR_BAD_SHAPE
+    for strides in ((128, 32, 1), (32, 32 * new, 1), (40, 40 * new, 1), (160, 40, 1)):  # rows or heads first, dense or not
+        assert torch.equal(be.attention_bf16(q, k, v, offsets([new]), offsets([200]), out=room.as_strided((new, 4, 32), strides)), want)
+    for t in (q[:1], q[:, :2].contiguous()):  # a dimension of one element has no stride
+        be.attention_bf16(t, k, v, offsets([len(t)]), offsets([200]), out=torch.empty_like(t))
