@@ -20,14 +20,18 @@
 // What bounds it: a block of a tile costs 1024 cycles of tensor pipe at width 128 (512 at 64) and 1024 of the exponential unit (16
 // per cycle), but the two tiles together take some 3200 cycles per block: a tile's softmax (1900) and the products between two
 // of them (1030) are a chain, as there is room for one block of scores per tile.  At width 128 and long prompts that is also
-// where the power limit sets the clock: 16 heads, 4 key heads, 16384 keys, causal: 855 us, 1290 TFLOP/s, 0.80 of the burst and
-// 0.96 of the sustained bf16 rate measured here; width 64: 771 us.  Prompts of a few hundred tokens spend as long at the items'
-// ends as in between: 64 sequences of 197, 16 heads of 64: 46 us, 0.35 of the bytes' rate.  There the softmax runs its first and
+// where the power limit sets the clock: 16 heads, 4 key heads, 16384 keys, causal: 857 us in a burst, 1283 TFLOP/s, 0.80 of the burst
+// bf16 rate measured here, and 982 us in calls that go on for seconds (1.63 GHz), 0.84 of the sustained one; width 64: 764 us.
+// Prompts of a few hundred tokens spend as long at the items' ends as in between: 64 sequences of 197, 16 heads of 64: 46 to 56 us
+// from one process to the next, 0.28 to 0.35 of the bytes' rate.  There the softmax runs its first and
 // masked blocks, whose code the warps do not have at hand (a fifth of their time went to waiting for instructions; a block took 2600
 // to 5200 cycles instead of 1900), while the output warps turn the item before around.  So what nobody needs is left out (tiles
 // without rows, warps whose rows are nobody's, the last quarter of a block that is seen half: 64 sequences of 128 keys of width 64,
 // 38 -> 31 us), and there is less code: the output warps' loop over the two tiles is rolled, and in the form for short prompts
-// (kShort) also that of the issuing warp, and an item's first block goes through the loop of the others (-> 27 us).
+// (kShort) also that of the issuing warp, and an item's first block goes through the loop of the others (-> 29 us).
+// Weights are rounded to bf16 for the second product, as their tensor's type has to be that of V: about as much as the bf16 result is
+// rounded itself (1.9e-3 to 2.3e-3 of the result, root mean square, against 64 bits; 1.5e-3 to 1.7e-3 with weights of 32 bits).  Two
+// bf16 terms would cost half as many products again.
 // Measured and not kept: scores of blocks of 64 keys two ahead (the instructions around twice as many blocks cost what the chain
 // does), an issuing warp per tile (the tiles fall into step: 1088 us).
 #include "attention_common.cuh"
@@ -761,9 +765,11 @@ int launch_form(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const
 template <int CH>
 int launch(swcb200_ctx *ctx, const Params &p, const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV, int tiles,
            int parts) {
-    // The form with less code up to 1024 keys per sequence.  Short against long form, 16384 tokens in sequences of one length, 32
+    // The form with less code up to 1024 keys per sequence: on average, as the lengths are on the device, and rows of a cache that are
+    // not filled count as keys.  Short against long form, 16384 tokens in sequences of one length, 32
     // heads, 8 key heads of 128, causal: 256 keys 111 / 115 us, 512 136 / 153, 1024 185 / 198, 2048 297 / 289; 16384 keys, 16 heads,
-    // 885 / 855.  Width 64, 16 heads, all keys: 64 sequences of 197 46 / 52 us, 32 of 1024 202 / 207.
+    // 885 / 855.  Width 64, 16 heads, all keys: 64 sequences of 197 46 / 52 us, 32 of 1024 202 / 207 (all of these before the row's
+    // Reference, which adds up to 1 %).  Under an SM limit the short one, whatever the length.
     const int blocks = tiles * p.units * parts, sms = swc_tc_sms(ctx);
     if (sms < ctx->sm_count && sms < blocks) return launch_form<CH, true, true>(ctx, p, tmQ, tmK, tmV, parts, blocks, sms);
     return p.total_k / p.batch <= 1024 ? launch_form<CH, true>(ctx, p, tmQ, tmK, tmV, parts, blocks, blocks)

@@ -11,8 +11,16 @@
 // mma.sync m16n8k16 on 16 of a block's 64 keys with a softmax of its own in registers -- no barrier between warps until the end
 // of an item, where the four key groups are merged.
 //
-// 32 heads, 8 key heads of 128, one token each: 64 caches of 4096 keys 173 us, 0.95 of the copy rate measured here; 64 ragged ones of up
-// to 4096 keys 64 us, 0.79 (CTAs that end apart); one cache of 65536 keys 50 us with its join, 0.82.
+// Weights go into the second product as bf16: its A operand has the type of B, the values.  That rounding (half a step is 2^-8 of a
+// weight, and the sum is of the unrounded ones) is about as large as the one of the bf16 result: 2.3e-3 of the result, root mean
+// square, against 64 bits, where weights of 32 bits would leave 1.7e-3.
+//
+// 32 heads, 8 key heads of 128, one token each: 64 caches of 4096 keys 171 us, 0.96 of the copy rate measured here; 64 ragged ones of up
+// to 4096 keys 64 us, 0.72 (items are dealt out by stride, and CTAs end apart); one cache of 65536 keys 50 us with its join, 0.82.
+// Slow by comparison: a sequence with more rows than fit the tile, which the AVERAGE number of rows sizes, has a CTA per row tile walk
+// all of its keys (16 new tokens behind 65536 keys beside 63 single ones: 777 us, 44 would do for the bytes); 64 rows per tile of
+// width 128 spill registers (64 caches of 2048 keys with 8 new tokens of 8 heads: 387 us, 85); thousands of sequences, as a search for
+// an item passes over all sequences before it (4096 caches of 256 keys: 4.5 ms, 0.67; 1024 of 512: 433 us, 332).
 #include "attention_common.cuh"
 
 namespace {

@@ -13,7 +13,8 @@
 //   would leave SMs idle; with few tokens it is bound by reading Wp once.
 // fc_res_pair_kernel: persistent CTA pairs (cta_group::2), 256 x BN tiles, two accumulators so that the epilogue of a tile runs
 //   beside the main loop of the next.  For everything else; bound by the tensor pipe: 16384 x 4096 x 4096 with bias, tanh-GELU and a
-//   bf16 residual 378 us, 1455 TFLOP/s, 0.91 of the burst rate of a library product measured here.
+//   bf16 residual 381 us in a burst, 1442 TFLOP/s, 0.90 of the burst rate of a library product measured here, and 441 us in calls that
+//   go on for seconds (1.28 GHz under the power limit), 0.93 of the sustained one.
 #include "tc_common.cuh"
 
 namespace {
@@ -592,7 +593,8 @@ struct Choice {
 // issuing threads, then loads), 0.30 in the pair form (the tensor pipe at 256 x 256); launch, first loads, epilogue 6.5 + 0.016 per
 // token; the join over 2 / 4 / 8 CTAs 0.8 / 2 / 3.5.  Forms compared in one run, (m, n) = (777, 1000): chosen 128 tokens over 2
 // CTAs 14.7 us; 4 CTAs (two waves) 21.6; undivided 19.9; 256 tokens over 4 18.1; pairs 26.1.  (64, 4096): 64 over 4 11.1; over 8
-// 12.4; undivided 17.7.
+// 12.4; undivided 17.7.  Different weights in every call, from HBM, and a bf16 residual, at n = k = 4096: 3 tokens 10.4 us, 16 10.6,
+// 64 13.3, 256 17.3; the bytes alone 5.2 to 6.1, and no weight is requested before the stream's previous kernel has ended.
 // limited: no more than `sms` CTAs at all, as each holds an SM of its own.  Only the pairs walk over tiles, so a split form is open
 // to calls of one wave; a limit of one SM gets a pair all the same.
 Choice choose(int m, int n, int kblocks, int sms, bool limited) {

@@ -9,9 +9,13 @@
 // (t - mean)^2 over the registers (no E[t^2] - mean^2, which cancels).  pre() reads t before it is rounded to sum's type:
 // the value is there, and rounding it first would only add an error to y.
 //
-// 65536 rows of 4096, gate, fp32 stream, layer norm: 570 us, 0.87 of the copy rate measured here.  8192 rows with RMS norms on both
-// sides, all bf16: 60 us, 0.68: two row sums one behind the other and 640 instructions a warp, half of the issue slots; requesting
-// whole rows ahead through shared memory (bulk copies, persistent CTAs) took 77 us and more.
+// 65536 rows of 4096, gate, fp32 stream, layer norm: 570 us, 0.87 of the copy rate measured here (629 us, 0.79, once calls have gone on
+// long enough for the power limit to take the clock to 1.76 GHz).  8192 rows with RMS norms on both
+// sides, all bf16: 61 us, 0.67: two row sums one behind the other, warps wait for loads and shared memory half of the time, and 61 % of
+// the issue slots are taken; requesting
+// whole rows ahead through shared memory (bulk copies, persistent CTAs) took 77 us and more.  Rows of odd width, read one element per
+// access, keep the issue slots busy instead (76 %): bf16, 20000 rows of 1003 63 us, 0.39; 50000 of 333 71 us, 0.29; 10000 of 4097, where
+// a thread's 17 elements take the form for 32, which spills, 239 us, 0.21.
 //
 // Layout: a row belongs to `tpr` threads.  Up to 32 of them (rows of at most 512 elements, 256 read singly) are a part of one
 // warp and the sums are shuffles; above that the row is a CTA of its own.  A thread holds at most 32 elements of a row.  Rows whose
