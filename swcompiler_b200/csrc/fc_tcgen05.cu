@@ -604,7 +604,8 @@ static int launch_fc(swcb200_ctx *ctx, bool pair, const CUtensorMap &tmA, const 
             attr_pair[dev] = true;
         }
         const long long tiles2 = (long long)p.tiles_m * p.tiles_n;
-        const long long max_clusters = swc_tc_sms(ctx) / 2;
+        const int sms = swc_tc_sms(ctx);
+        const long long max_clusters = sms > 1 ? sms / 2 : 1;  // a limit of one SM gets a pair all the same
         unsigned grid2 = 2u * (unsigned)(tiles2 < max_clusters ? tiles2 : max_clusters);
         fc_tc_pair_kernel<SPLIT><<<grid2, kThreads, Pair<SPLIT>::kSmemBytes, ctx->stream>>>(tmA, tmAlo, tmB, p);
         return swc_check_launch(ctx, "fc_bf16");

@@ -215,3 +215,16 @@ def test_attention_outputs_that_overlap_themselves_are_refused(be, new):
         assert torch.equal(be.attention_bf16(q, k, v, offsets([new]), offsets([200]), out=room.as_strided((new, 4, 32), strides)), want)
     for t in (q[:1], q[:, :2].contiguous()):  # a dimension of one element has no stride
         be.attention_bf16(t, k, v, offsets([len(t)]), offsets([200]), out=torch.empty_like(t))
+
+
+@pytest.mark.parametrize("limit", [1, 2, 3])
+def test_fc_bf16_under_the_smallest_sm_limits(be, limit):
+    rn = gen(limit)
+    a, wp = rn(700, 256, dtype=BF16), rn(900, 256, dtype=BF16, s=256 ** -0.5)
+    be.set_sm_limit(limit)
+    try:
+        fc_check(be.fc_bf16(a, wp, out_dtype=F32), a, wp, None, "NONE", None, 1.0)
+        fc_check(be.fc_bf16_residual(a, wp, out_dtype=F32), a, wp, None, "NONE", None, 1.0)
+    finally:
+        be.set_sm_limit(0)
+    be.sync()
